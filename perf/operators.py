@@ -4,7 +4,8 @@ plain form in elementary torch operations.
 * ``verify``: ``requests`` requests bring up to ``drafts`` drafted tokens each and rows of logits over ``vocab`` tokens. Which
   drafts hold, and the token that follows them, by the request's temperature, top-k threshold and random stream. ``kind``:
   ``greedy``, ``sampled``, or ``mixed`` (of four requests one is greedy, one has no top-k threshold). ``draft_logits``: the drafts
-  were drawn by a model whose logits are there too; otherwise they come from a lookup and are certain.
+  were drawn by a model whose logits are there too, and hold by the ratio of the probabilities; otherwise they come from a lookup,
+  and hold where they are what the stream draws.
 * ``ngram``: ``requests`` requests with texts of up to ``context`` tokens take up to ``drafts`` + 1 verified tokens in and get
   drafts that followed the latest longest match (at most ``match`` tokens) of their last tokens.
 * ``arrays``: positions, owners, slots, attention tiles and block tables of a step to which ``requests`` requests bring up to
@@ -234,6 +235,19 @@ def _uniform(word):                          # in (0, 1), exact in 32 bits
     return ((word >> 9).to(torch.float32) + 0.5) * (1.0 / 8388608.0)
 
 
+def _noise_words(v, seed, step, stream, domain):
+    """Row by row a word per token; seed, step, stream and domain are columns."""
+    blocks = torch.arange((v + 3) // 4, device=seed.device)[None, :]
+    words = _philox(*torch.broadcast_tensors(blocks, step, stream, domain), seed)
+    return torch.stack(words, dim=2).reshape(seed.shape[0], -1)[:, :v]
+
+
+def _noisy(s, seed, step, stream):
+    """Scaled logits with the Gumbel noise of their row's stream."""
+    words = _noise_words(s.shape[1], seed, step, stream, torch.zeros_like(step))
+    return s - torch.log(-torch.log(_uniform(words)))
+
+
 def _scaled(x, temperature, topk, kmax):
     """Rows over their temperature, what the threshold drops and what is no number at -inf."""
     s = x / temperature[:, None]
@@ -292,31 +306,29 @@ def _plain_verify(st):
     a = torch.where(greedy[owner[before]], (drafted == best[before]).double(), a)
     accept = torch.zeros((n_req, d), dtype=torch.float64, device=logits.device)
     accept[owner[before], place[before]] = a
+    if st["draft_logits"] is None:
+        # what the stream draws for every row
+        owner_ = owner[:, None]
+        drawn = _noisy(s, st["seed"][owner_], st["step"].long()[owner_] + place[:, None], st["stream_id"].long()[owner_]).argmax(1)
+        drawn = torch.where(greedy[owner], best, drawn)
+        holds = torch.zeros((n_req, d), dtype=torch.int64, device=logits.device)
+        holds[owner[before], place[before]] = (drawn[before] == drafted).long()
+        held = holds.cumprod(1).sum(1)
+        return dict(tokens=_emitted(st, cu, held, drawn[cu[:-1] + held]), counts=(held + 1).int(), accept=accept.float())
     seed, stream, step = st["seed"][:, None], st["stream_id"].long()[:, None], st["step"].long()[:, None]
     j = torch.arange(d, device=logits.device)[None, :]
     u = _uniform(_philox(torch.zeros_like(step + j), step + j, stream.expand(-1, d), torch.ones_like(step + j), seed.expand(-1, d))[0])
     held = (u < accept).int().cumprod(1).sum(1)
-    last = cu[:-1] + held                                            # the row that the next token is drawn from
-    rejected = held < cu[1:] - cu[:-1] - 1
-    # the draw: noise per (request, position, token)
-    at = last.clamp(max=logits.shape[0] - 1)
-    refused = st["token_ids"][(at + 1).clamp(max=logits.shape[0] - 1)].long()
-    with_q = st["draft_logits"] is not None
-    domain = torch.where(rejected & with_q, 2, 0)[:, None]
-    blocks = torch.arange((v + 3) // 4, device=logits.device)[None, :].expand(n_req, -1)
-    words = torch.stack(_philox(*torch.broadcast_tensors(blocks, step + held[:, None], stream, domain), seed), dim=2).reshape(n_req, -1)[:, :v]
-    e = -torch.log(_uniform(words))
-    score = s[at] - torch.log(e)
-    struck = (rejected & ~torch.tensor(with_q, device=logits.device))[:, None] & (torch.arange(v, device=logits.device)[None, :] == refused[:, None])
-    score = torch.where(struck, -math.inf, score)
-    if with_q:
-        row_of = torch.zeros((logits.shape[0],), dtype=torch.int64, device=logits.device)
-        row_of[before] = torch.arange(len(before), device=logits.device)
-        pr = (w[at] / z[at][:, None]).float()
-        qr = (dw[row_of[at]] / dz[row_of[at]][:, None]).float() if len(before) else torch.zeros_like(pr)
-        left = (pr - qr).clamp(min=0.0)
-        left = torch.where((left > 0).any(1, keepdim=True), left, pr)
-        score = torch.where(rejected[:, None], torch.where(left > 0, left / e, -math.inf), score)
+    at = cu[:-1] + held                                              # the row that the next token is drawn from
+    rejected = (held < cu[1:] - cu[:-1] - 1)[:, None]
+    row_of = torch.zeros((logits.shape[0],), dtype=torch.int64, device=logits.device)
+    row_of[before] = torch.arange(len(before), device=logits.device)
+    pr = (w[at] / z[at][:, None]).float()
+    qr = (dw[row_of[at]] / dz[row_of[at]][:, None]).float() if len(before) else pr
+    left = (pr - qr).clamp(min=0.0)
+    left = torch.where((left > 0).any(1, keepdim=True), left, pr)
+    e = -torch.log(_uniform(_noise_words(v, seed, step + held[:, None], stream, torch.where(rejected, 2, 0))))
+    score = torch.where(rejected, torch.where(left > 0, left / e, -math.inf), s[at] - torch.log(e))
     drawn = torch.where(greedy, best[at], score.argmax(1))
     return dict(tokens=_emitted(st, cu, held, drawn), counts=(held + 1).int(), accept=accept.float())
 
@@ -424,6 +436,16 @@ def _distribution64(row, temperature, k):
     return torch.softmax(torch.where(drop, -math.inf, x / float(temperature)), 0)
 
 
+def _drawn64(st, r, row, place):
+    """The token that request r's stream draws from a row of logits."""
+    x = st["logits"][row]
+    if int(st["greedy"][r]):
+        return int(x.argmax())
+    p = _distribution64(x, st["temperature"][r], int(st["topk"][r]))
+    u = _words64(np.arange((len(x) + 3) // 4), int(st["step"][r]) + place, int(st["stream_id"][r]), 0, int(st["seed"][r]))[:len(x)]
+    return int((p.log() - (-torch.from_numpy(u).to(p.device).log()).log()).argmax())
+
+
 def _exact_verify(st):
     cu, fed = st["cu_rows"].tolist(), st["token_ids"].tolist()
     n_req, d, v = len(cu) - 1, st["drafts"], st["vocab"]
@@ -431,7 +453,7 @@ def _exact_verify(st):
     counts = torch.zeros(n_req, dtype=torch.int32)
     accept = torch.zeros((n_req, d), dtype=torch.float64)
     seeds, streams, steps = st["seed"].tolist(), st["stream_id"].tolist(), st["step"].tolist()
-    greedy, topk = st["greedy"].tolist(), st["topk"].tolist()
+    greedy, topk, with_q = st["greedy"].tolist(), st["topk"].tolist(), st["draft_logits"] is not None
     for r in range(n_req):
         t, n, held = st["temperature"][r], cu[r + 1] - cu[r] - 1, None
         for j in range(n):
@@ -442,23 +464,20 @@ def _exact_verify(st):
                 p = float(_distribution64(row, t, topk[r])[draft])
                 q = 1.0 if st["draft_logits"] is None else float(_distribution64(st["draft_logits"][r, j], t, topk[r])[draft])
                 accept[r, j] = min(1.0, p / q) if q > 0 else float(p > 0)
-            if held is None and not _words64([0], steps[r] + j, streams[r], 1, seeds[r])[0] < float(accept[r, j]):
+            if held is None and with_q and not _words64([0], steps[r] + j, streams[r], 1, seeds[r])[0] < float(accept[r, j]):
+                held = j
+            if held is None and not with_q and _drawn64(st, r, cu[r] + j, j) != draft:
                 held = j
         refused = held is not None
         held = n if held is None else held
-        row = st["logits"][cu[r] + held]
-        if greedy[r]:
-            token = int(row.argmax())
+        if refused and with_q and not greedy[r]:
+            p = _distribution64(st["logits"][cu[r] + held], t, topk[r])
+            q = _distribution64(st["draft_logits"][r, held], t, topk[r])
+            p = torch.where(p > q, p - q, 0.0) if bool((p > q).any()) else p
+            u = torch.from_numpy(_words64(np.arange((v + 3) // 4), steps[r] + held, streams[r], 2, seeds[r])[:v]).to(p.device)
+            token = int((p.log() - (-u.log()).log()).argmax())
         else:
-            p = _distribution64(row, t, topk[r])
-            with_q = refused and st["draft_logits"] is not None
-            if with_q:
-                q = _distribution64(st["draft_logits"][r, held], t, topk[r])
-                p = torch.where(p > q, p - q, 0.0) if bool((p > q).any()) else p
-            elif refused:
-                p[fed[cu[r] + held + 1]] = 0.0
-            u = _words64(np.arange((v + 3) // 4), steps[r] + held, streams[r], 2 if with_q else 0, seeds[r])[:v]
-            token = int((p.log() - (-torch.from_numpy(u).to(p.device).log()).log()).argmax())
+            token = _drawn64(st, r, cu[r] + held, held)
         tokens[r, :held] = torch.tensor(fed[cu[r] + 1:cu[r] + 1 + held], dtype=torch.int32)
         tokens[r, held] = token
         counts[r] = held + 1
