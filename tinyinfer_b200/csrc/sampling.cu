@@ -6,35 +6,10 @@
 // Philox-4x32-10 block with counter (i / 4, step, stream, 0) and key (seed), so a row's token
 // depends only on (seed, stream, step) and its logits, whatever else is in the batch.
 #include "common.cuh"
+#include "draws.cuh"
 
 constexpr int SP_THREADS = 256;      // argmax parts, nll
 
-__device__ __forceinline__ uint4 philox4x32_10(uint4 c, uint2 k) {
-#pragma unroll
-    for (int r = 0; r < 10; ++r) {
-        const unsigned hi0 = __umulhi(0xD2511F53u, c.x), lo0 = 0xD2511F53u * c.x;
-        const unsigned hi1 = __umulhi(0xCD9E8D57u, c.z), lo1 = 0xCD9E8D57u * c.z;
-        c = make_uint4(hi1 ^ c.y ^ k.x, lo1, hi0 ^ c.w ^ k.y, lo0);
-        k.x += 0x9E3779B9u;
-        k.y += 0xBB67AE85u;
-    }
-    return c;
-}
-__device__ __forceinline__ float philox_uniform(unsigned word) {   // in (0, 1), exact in float32
-    return ((float)(word >> 9) + 0.5f) * (1.0f / 8388608.0f);
-}
-__device__ __forceinline__ unsigned order_key(float v) {           // larger float -> larger key
-    const unsigned b = __float_as_uint(v);
-    return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
-}
-
-struct Best { float v; int i; };
-__device__ __forceinline__ Best better(Best a, Best b) {
-    if (b.i < 0) return a;
-    if (a.i < 0) return b;
-    if (b.v > a.v || (b.v == a.v && b.i < a.i)) return b;
-    return a;
-}
 __device__ __forceinline__ Best block_best(Best x, Best* sh) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
@@ -103,76 +78,6 @@ __device__ __forceinline__ void for_each_logit(const float* x, int vocab, int be
     }
 }
 
-// Radix select, one byte per pass from the top: the k-th largest of the keys that `each` hands out (it calls
-// its argument once per key; every thread of the block calls select_kth with the same k). 0 if k <= 0.
-// hist: 256 shared words; sel: 2 shared words. The counts of a pass go into the histogram warp by warp: lanes
-// that hold the same byte count themselves once together (most logits share their sign and exponent, so a
-// plain atomic per key would make a warp wait for itself 32 times over); the bin that holds the k-th largest
-// is found by the first warp together (a suffix sum over lanes of eight bins each), not by one thread.
-// One pass: sel[0] holds the bytes found so far (from the top), sel[1] which of the keys that begin with them,
-// counted from the largest, is looked for; afterwards one byte more and the rank among those.
-template <typename Each>
-__device__ __forceinline__ void radix_pass(int pass, unsigned* hist, unsigned* sel, Each each) {
-    {
-        const int shift = 24 - 8 * pass;
-        for (int i = threadIdx.x; i < 256; i += blockDim.x) hist[i] = 0u;
-        __syncthreads();
-        const unsigned prefix = sel[0];
-        const unsigned mask = pass == 0 ? 0u : (0xFFFFFFFFu << (shift + 8));
-        each([&](unsigned key) {
-            if ((key & mask) == prefix) {
-                const unsigned bin = (key >> shift) & 0xFFu;
-                const unsigned same = __match_any_sync(__activemask(), bin);
-                if ((threadIdx.x & 31) == (unsigned)(__ffs(same) - 1)) atomicAdd(&hist[bin], (unsigned)__popc(same));
-            }
-        });
-        __syncthreads();
-        if (threadIdx.x < 32) {
-            const int lane = threadIdx.x;
-            unsigned mine[8], sum = 0u;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) { mine[i] = hist[8 * lane + i]; sum += mine[i]; }
-            unsigned above = sum;                                  // keys in this lane's bins and all higher ones
-#pragma unroll
-            for (int off = 1; off < 32; off <<= 1) {
-                const unsigned v = __shfl_down_sync(0xffffffffu, above, off);
-                if (lane + off < 32) above += v;
-            }
-            const unsigned remaining = sel[1];
-            // the highest lane whose bins, with all above them, reach the k-th largest; lane 0 if none does
-            const unsigned reach = __ballot_sync(0xffffffffu, above >= remaining);
-            const int owner = reach ? 31 - __clz(reach) : 0;
-            if (lane == owner) {
-                unsigned left = remaining - (above - sum);         // still to find inside this lane's bins
-                int b = 7;
-                if (reach) {
-                    for (; b > 0; --b) {
-                        if (mine[b] >= left) break;
-                        left -= mine[b];
-                    }
-                } else {
-                    b = 0;                                         // fewer keys than k: bin 0, as the plain walk does
-                    left = remaining;
-                    for (int i = 255; i > 0; --i) left -= hist[i];
-                }
-                sel[0] = prefix | ((unsigned)(8 * lane + b) << shift);
-                sel[1] = left;
-            }
-        }
-        __syncthreads();
-    }
-}
-template <typename Each>
-__device__ __forceinline__ unsigned select_kth(int k, unsigned* hist, unsigned* sel, Each each) {
-    if (k <= 0) return 0u;
-    if (threadIdx.x == 0) { sel[0] = 0u; sel[1] = (unsigned)k; }
-    for (int pass = 0; pass < 4; ++pass) radix_pass(pass, hist, sel, each);
-    return sel[0];
-}
-
-__device__ __forceinline__ float key_value(unsigned key) {          // the inverse of order_key
-    return __uint_as_float((key & 0x80000000u) ? (key & 0x7FFFFFFFu) : ~key);
-}
 __device__ __forceinline__ float gumbel(int index, unsigned c1, unsigned c2, uint2 key2) {
     const uint4 r = philox4x32_10(make_uint4((unsigned)(index >> 2), c1, c2, 0u), key2);
     const unsigned words[4] = {r.x, r.y, r.z, r.w};
