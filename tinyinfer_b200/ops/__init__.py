@@ -12,7 +12,7 @@ from __future__ import annotations
 
 import array
 import ctypes
-from typing import Optional, Sequence
+from typing import NamedTuple, Optional, Sequence
 
 import torch
 
@@ -26,6 +26,14 @@ class KernelError(RuntimeError):
 
 
 _SIGNATURES = {
+    "drafts": {
+        "ti_verify_drafts": [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_void_p, c_void_p,
+                             c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_ll, c_ll, c_void_p, c_void_p],
+        "ti_verify_scratch_words": [c_int, c_int, c_int],
+        "ti_ngram_drafts": [c_void_p] * 11 + [c_int] * 7 + [c_void_p],
+        "ti_step_arrays": [c_void_p] * 15 + [c_int] * 9 + [c_void_p],
+        "ti_step_tile_rows": [],
+    },
     "core": {
         "ti_embedding": [c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_void_p],
         "ti_feed_tokens": [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p],
@@ -239,7 +247,11 @@ def status_message(wait_code: int, page_code: int) -> Optional[str]:
                     "the step's results are not to be used")
     elif wait_code:
         said.append(f"a kernel gave up waiting on a barrier (status {wait_code}); the step's results are not to be used")
-    if page_code:
+    if page_code == 5:
+        said.append("the requests of a step brought more tokens than its arrays have room for; what did not fit is missing from it")
+    elif page_code == 6:
+        said.append("a request's text has no row in the history, or outgrew it; the request sat the step out")
+    elif page_code:
         said.append(f"a kernel met a token or key without a page (status {page_code})")
     return "; ".join(said) or None
 
@@ -2342,6 +2354,229 @@ def sample(logits: torch.Tensor, temperature: torch.Tensor, topk: torch.Tensor, 
          temperature.data_ptr(), topk.data_ptr(), greedy.data_ptr(), seed.data_ptr(),
          stream_id.data_ptr(), step.data_ptr(), *(t.data_ptr() for t in scratch), _ptr(extra), num_extra, _stream())
     return out
+
+
+# ---------------------------------------------------------------------- decoding with drafts
+MAX_DRAFTS = 31           # drafts a request and step: a warp of the verification decides a request, a lane a draft
+
+
+class VerifiedDrafts(NamedTuple):
+    tokens: torch.Tensor      # int32 [S, max_drafts + 1]: the drafts that held, the token drawn behind them, then -1
+    counts: torch.Tensor      # int32 [S]: how many tokens that is (0: the request has no rows)
+    accept: torch.Tensor      # float32 [S, max_drafts]: how likely each draft was to hold (0 where there is none)
+
+
+class NgramDrafts(NamedTuple):
+    tokens: torch.Tensor      # int32 [S, max_drafts + 1]: the last token of each text, its drafts, then -1
+    counts: torch.Tensor      # int32 [S]: how many tokens that is (0: no text)
+    starts: torch.Tensor      # int32 [S]: the position of the first of them
+    lengths: torch.Tensor     # int32 [S]: the texts' lengths, the new tokens among them
+
+
+class StepArrays(NamedTuple):
+    token_ids: Optional[torch.Tensor]     # int32 [rows], None without tokens
+    positions: torch.Tensor               # int32 [rows]
+    token_seq: torch.Tensor               # int32 [rows]
+    cache_slots: torch.Tensor             # int32 [groups, rows]: page * page_size + position % page_size, -1 without a page
+    cu_seqlens: torch.Tensor              # int32 [S + 2]
+    q_starts: torch.Tensor                # int32 [S + 1]
+    context_lens: torch.Tensor            # int32 [S + 1]
+    tiles: torch.Tensor                   # int32 [S * ceil(max_count / 128), 4]
+    block_tables: torch.Tensor            # int32 [groups, S + 1, width]
+
+
+def _on_current(device) -> None:
+    if device.index != torch.cuda.current_device():
+        raise KernelError(f"the tensors lie on {device}, the current device is cuda:{torch.cuda.current_device()}")
+
+
+def _per_request(n: int, device, **tensors) -> None:
+    """Checks tensors of one entry a request on one device."""
+    for name, (t, dtype) in tensors.items():
+        _check(t, name, dtype, 1)
+        if t.shape[0] != n:
+            raise KernelError(f"{name} must have one entry per request: {n}, got {t.shape[0]}")
+        if t.device != device:
+            raise KernelError(f"{name} lies on {t.device}, the others on {device}")
+
+
+def verify_drafts(logits: torch.Tensor, token_ids: torch.Tensor, cu_rows: torch.Tensor, *, max_drafts: int,
+                  temperature: Optional[torch.Tensor] = None, topk: Optional[torch.Tensor] = None,
+                  greedy: Optional[torch.Tensor] = None, seed: Optional[torch.Tensor] = None,
+                  stream_id: Optional[torch.Tensor] = None, step: Optional[torch.Tensor] = None,
+                  draft_logits: Optional[torch.Tensor] = None) -> VerifiedDrafts:
+    """Which drafted tokens hold, and the token behind them. Request r brought the tokens ``token_ids[cu_rows[r] : cu_rows[r + 1]]``
+    (int32 [N]; ``cu_rows`` int32 [S + 1]), one that is settled and up to ``max_drafts`` drafts, and ``logits`` float32 [N, V] has the
+    row behind each: row j judges draft j, the last row is for the token behind all of them. Rows past ``max_drafts + 1`` of a request
+    and rows that no request claims are not looked at; a request without rows gets no token.
+
+    The sampling options are those of ``sample``, one entry per request; ``step`` counts for the request's first row, row j draws at
+    step + j. Without any of them every request is greedy. Without ``draft_logits`` a draft holds where it is the token that ``sample``
+    (greedy: ``argmax``) gives for its row, and behind the first that does not, that token follows: what comes out is what decoding
+    one by one with the same streams gives. With ``draft_logits`` (float32 [S, max_drafts, V], any strides but the last) the drafts of
+    sampled requests were drawn from them, under the same temperature and top-k, and draft j holds with probability min(1, p / q), p and
+    q its shares of the two softmaxes over what temperature and top-k keep; behind the first that fails the token is drawn from what is
+    left of p beyond q, and if all hold it is the one that ``sample`` gives for the last row: the tokens are distributed as if ``sample``
+    had drawn them one by one. ``accept`` of the result: min(1, p / q), without ``draft_logits`` p, of greedy requests 1 or 0.
+    All random numbers are functions of (seed, stream_id, step + j): a result does not depend on the rest of the batch. Those that judge
+    drafts and that draw behind one that failed against ``draft_logits`` are apart from the noise of ``sample``, which the drafts may
+    have been drawn with.
+
+    A draft outside the vocabulary never holds. NaN logits are passed over, as ``sample`` does; a sampled row with nothing but NaN and
+    -inf lets no draft hold and gives token 0."""
+    _check(logits, "logits", torch.float32, 2)
+    _check(token_ids, "token_ids", torch.int32, 1)
+    _check(cu_rows, "cu_rows", torch.int32, 1)
+    n, vocab = logits.shape
+    s, d, device = cu_rows.shape[0] - 1, int(max_drafts), logits.device
+    if s < 0 or token_ids.shape[0] != n or vocab < 1:
+        raise KernelError(f"verify_drafts: {tuple(logits.shape)} logits, {token_ids.shape[0]} tokens, cu_rows of {s + 1} entries")
+    if not 0 <= d <= MAX_DRAFTS:
+        raise KernelError(f"verify_drafts: max_drafts must be 0 to {MAX_DRAFTS}, got {d}")
+    if token_ids.device != device or cu_rows.device != device:
+        raise KernelError("verify_drafts: all tensors lie on one device")
+    options = (temperature, topk, greedy, seed, stream_id, step)
+    given = sum(t is not None for t in options)
+    if given not in (0, 6):
+        raise KernelError("verify_drafts: the sampling options go together: temperature, topk, greedy, seed, stream_id, step")
+    stride_s = stride_d = 0
+    if given:
+        _per_request(s, device, temperature=(temperature, torch.float32), topk=(topk, torch.int32), greedy=(greedy, torch.int32),
+                     seed=(seed, torch.int64), stream_id=(stream_id, torch.int32), step=(step, torch.int32))
+    if draft_logits is not None:
+        if not given:
+            raise KernelError("verify_drafts: without sampling options every request is greedy and draft_logits have no use")
+        if draft_logits.dtype != torch.float32 or draft_logits.device != device:
+            raise KernelError(f"draft_logits must be float32 on {device}, got {draft_logits.dtype} on {draft_logits.device}")
+        if tuple(draft_logits.shape) != (s, d, vocab) or (draft_logits.numel() and vocab > 1 and draft_logits.stride(2) != 1):
+            raise KernelError(f"draft_logits must be [{s}, {d}, {vocab}] with neighbouring tokens side by side, got "
+                              f"{tuple(draft_logits.shape)} with strides {draft_logits.stride()}")
+        stride_s, stride_d = draft_logits.stride(0), draft_logits.stride(1)
+        if d == 0:
+            draft_logits = None
+    _on_current(device)
+    out = VerifiedDrafts(torch.empty((s, d + 1), dtype=torch.int32, device=device), torch.empty((s,), dtype=torch.int32, device=device),
+                         torch.empty((s, d), dtype=torch.float32, device=device))
+    # scratch of the call's own: calls on several streams, or in several captured graphs, do not meet in it
+    scratch = torch.empty((_verify_scratch_words(s, d, vocab),), dtype=torch.int32, device=device)
+    _run("drafts", "ti_verify_drafts", out.tokens.data_ptr(), out.counts.data_ptr(), out.accept.data_ptr(), logits.data_ptr(),
+         token_ids.data_ptr(), cu_rows.data_ptr(), n, vocab, s, d, *(_ptr(t) for t in options), _ptr(draft_logits), stride_s, stride_d,
+         scratch.data_ptr(), _stream())
+    return out
+
+
+def _verify_scratch_words(requests: int, max_drafts: int, vocab: int) -> int:
+    key = ("verify", requests, max_drafts, vocab)
+    n = _scratch_floats.get(key)
+    if n is None:
+        fn = _fn("drafts", "ti_verify_scratch_words")
+        fn.restype = ctypes.c_longlong
+        n = _scratch_floats[key] = int(fn(requests, max_drafts, vocab))
+    return n
+
+
+def ngram_drafts(history: torch.Tensor, lengths: torch.Tensor, *, max_drafts: int, max_match: int = 3, min_match: int = 1,
+                 tokens: Optional[torch.Tensor] = None, counts: Optional[torch.Tensor] = None,
+                 state_slots: Optional[torch.Tensor] = None, limits: Optional[torch.Tensor] = None,
+                 status: Optional[torch.Tensor] = None) -> NgramDrafts:
+    """Drafts from each request's own text: what followed where its last tokens stood before. ``history`` int32 [M, L] holds the texts,
+    request i's in row ``state_slots[i]`` (int32 [S]; None: row i), ``lengths`` int32 [S] their lengths. ``tokens`` int32 [S, C] with
+    ``counts`` int32 [S] (what ``verify_drafts`` returned, say) are first written behind the texts; ``lengths`` is left alone and the
+    new lengths are returned, so a call made twice does the same twice. A request that brings tokens has a row to itself.
+
+    Of the earlier places where the text's last ``max_match`` tokens, or as many of them as possible, at least ``min_match``, stood, the
+    latest with the longest match is taken; the drafts are the tokens that followed there, and where the text ends, the drafts' own
+    beginning (a repetition shorter than the drafts goes round). ``limits`` int32 [S]: most drafts of a request, below ``max_drafts``.
+    The result's ``tokens`` start with the text's last token: with ``counts`` and ``starts`` they are what ``step_arrays`` takes for
+    a request whose cache holds all but its last token. A request whose row does not exist, or whose text is longer than it,
+    sits out (count 0) and sets the ``status`` word."""
+    _check(history, "history", torch.int32, 2)
+    device = history.device
+    _check(lengths, "lengths", torch.int32, 1)
+    s, d = lengths.shape[0], int(max_drafts)
+    _per_request(s, device, lengths=(lengths, torch.int32))
+    if not 0 <= d <= MAX_DRAFTS:
+        raise KernelError(f"ngram_drafts: max_drafts must be 0 to {MAX_DRAFTS}, got {d}")
+    if not 1 <= min_match <= max_match <= 32:
+        raise KernelError(f"ngram_drafts: 1 <= min_match <= max_match <= 32, got {min_match} and {max_match}")
+    if state_slots is None and history.shape[0] < s:
+        raise KernelError(f"ngram_drafts: {s} requests, but the history has {history.shape[0]} rows")
+    if (tokens is None) != (counts is None):
+        raise KernelError("ngram_drafts: tokens and counts go together")
+    if tokens is not None:
+        _check(tokens, "tokens", torch.int32, 2)
+        if tokens.shape[0] != s or tokens.shape[1] > 512 or tokens.device != device:
+            raise KernelError(f"ngram_drafts: tokens must be [{s}, at most 512] on {device}, got {tuple(tokens.shape)} on {tokens.device}")
+    optional = dict(counts=counts, state_slots=state_slots, limits=limits)
+    _per_request(s, device, **{name: (t, torch.int32) for name, t in optional.items() if t is not None})
+    if status is not None:
+        _check(status, "status", torch.int32, 1)
+    _on_current(device)
+    out = NgramDrafts(torch.empty((s, d + 1), dtype=torch.int32, device=device), *torch.empty((3, s), dtype=torch.int32, device=device))
+    _run("drafts", "ti_ngram_drafts", out.tokens.data_ptr(), out.counts.data_ptr(), out.starts.data_ptr(), out.lengths.data_ptr(),
+         history.data_ptr(), lengths.data_ptr(), _ptr(state_slots), _ptr(tokens), _ptr(counts), _ptr(limits), _ptr(status), s,
+         history.shape[0], history.shape[1], tokens.shape[1] if tokens is not None else 0, d, int(min_match), int(max_match), _stream())
+    return out
+
+
+def step_arrays(starts: torch.Tensor, counts: torch.Tensor, block_tables: torch.Tensor, *, rows: int, max_count: int, page_size: int,
+                tokens: Optional[torch.Tensor] = None, state_slots: Optional[torch.Tensor] = None, pad_page: int = -1,
+                status: Optional[torch.Tensor] = None) -> StepArrays:
+    """The arrays of a step, built on the device from lengths that the host need not know: request s has ``starts[s]`` tokens stored and
+    brings ``counts[s]`` (int32 [S], 0: none), at most ``max_count``, the first of ``tokens[s]`` (int32 [S, >= max_count]; None: no
+    ``token_ids`` are made). ``block_tables`` int32 [groups, M, width] (or [M, width]: one group) holds the pages of every request,
+    request s's in row ``state_slots[s]`` (int32 [S]; None: row s): as many as its tokens need, -1 where it has none.
+
+    The result has ``rows`` flat rows, whatever the counts: the requests' tokens one after the other, and behind them rows of a
+    request number S at position 0 with the one page ``pad_page``, which no other request holds (-1: none), so that a step of a fixed size
+    can be captured. Their ``cache_slots`` are -1. ``cu_seqlens``: the requests' first rows, that of number S, ``rows``. ``tiles``: up to
+    128 rows each, ``ceil(max_count / 128)`` per request, [request, first row, rows (0: none), first position], as the one-tile attention
+    kernels take them. ``block_tables``: the pages up to each request's end, -1 behind them, number S's last.
+
+    What does not fit into ``max_count`` or ``rows``, and a request whose row or start does not exist, is left out and sets the
+    ``status`` word, as a token without a page does (``page_status``)."""
+    _check(starts, "starts", torch.int32, 1)
+    s, device = starts.shape[0], starts.device
+    _per_request(s, device, starts=(starts, torch.int32), counts=(counts, torch.int32))
+    if state_slots is not None:
+        _per_request(s, device, state_slots=(state_slots, torch.int32))
+    if block_tables.dim() == 2:
+        block_tables = block_tables.unsqueeze(0)
+    _check(block_tables, "block_tables", torch.int32, 3)
+    groups, table_rows, width = block_tables.shape
+    if groups < 1 or width < 1 or block_tables.device != device:
+        raise KernelError(f"step_arrays: block_tables must be [groups, requests, pages] on {device}, got {tuple(block_tables.shape)} on "
+                          f"{block_tables.device}")
+    if state_slots is None and table_rows < s:
+        raise KernelError(f"step_arrays: {s} requests, but the block tables have {table_rows} rows")
+    if rows < 0 or max_count < 1 or page_size < 1:
+        raise KernelError(f"step_arrays: bad sizes: rows {rows}, max_count {max_count}, page_size {page_size}")
+    if tokens is not None:
+        _check(tokens, "tokens", torch.int32, 2)
+        if tokens.shape[0] != s or tokens.shape[1] < max_count or tokens.device != device:
+            raise KernelError(f"step_arrays: tokens must be [{s}, at least {max_count}] on {device}, got {tuple(tokens.shape)} on "
+                              f"{tokens.device}")
+    if status is not None:
+        _check(status, "status", torch.int32, 1)
+    _on_current(device)
+    tiles = s * -(-max_count // STEP_TILE)
+    sizes = [4 * tiles, groups * (s + 1) * width, groups * rows, rows, rows, rows if tokens is not None else 0, s + 2, s + 1, s + 1]
+    starts_at, total = [], 0
+    for words in sizes:                                  # one allocation; every array starts on a 16-byte boundary
+        starts_at.append(total)
+        total += (words + 3) // 4 * 4
+    buf = torch.empty((total,), dtype=torch.int32, device=device)
+    tile_v, table_v, slot_v, pos_v, seq_v, id_v, cu_v, start_v, ctx_v = (buf[at:at + words] for at, words in zip(starts_at, sizes))
+    out = StepArrays(id_v if tokens is not None else None, pos_v, seq_v, slot_v.view(groups, rows), cu_v, start_v, ctx_v,
+                     tile_v.view(tiles, 4), table_v.view(groups, s + 1, width))
+    _run("drafts", "ti_step_arrays", _ptr(out.token_ids), pos_v.data_ptr(), seq_v.data_ptr(), slot_v.data_ptr(), cu_v.data_ptr(),
+         start_v.data_ptr(), ctx_v.data_ptr(), tile_v.data_ptr(), table_v.data_ptr(), starts.data_ptr(), counts.data_ptr(),
+         _ptr(state_slots), block_tables.data_ptr(), _ptr(tokens), _ptr(status), s, groups, table_rows, width,
+         tokens.shape[1] if tokens is not None else 0, int(rows), int(max_count), int(page_size), int(pad_page), _stream())
+    return out
+
+
+STEP_TILE = 128           # query rows of the tiles that step_arrays makes: the one-tile attention kernels'
 
 
 def token_nll(logits: torch.Tensor, tokens: torch.Tensor) -> torch.Tensor:

@@ -35,7 +35,10 @@ LIBRARIES: Dict[str, dict] = {
     # every dtype, every shape: the 32-bit path and the general bfloat16 path of the plain decoder, and sampling
     "core": dict(sources=["runtime.cu", "elementwise.cu", "rope_append.cu",
                           "attention_generic.cu", "gemm_simt.cu", "sampling.cu"],
-                 headers=["common.cuh"], link=[]),
+                 headers=["common.cuh", "draws.cuh"], link=[]),
+    # decoding with drafts: verification, drafts from the request's own text, a step's arrays from lengths on the device
+    "drafts": dict(sources=["runtime.cu", "verify_drafts.cu", "ngram_drafts.cu", "step_arrays.cu"], headers=["common.cuh", "draws.cuh"],
+                   link=[]),
     # a dense decoder's layers launched from one call, through the other libraries' launchers
     "stack": dict(sources=["runtime.cu", "dense_stack.cu"], headers=["common.cuh"], link=[]),
     # the 32-bit path at the sizes it is used at: products and attention
