@@ -22,6 +22,24 @@ __device__ __forceinline__ unsigned order_key(float v) {           // larger flo
     return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
 }
 
+// Launches `kernel` on clusters of `ctas` blocks along x (more than 8: the kernel has to allow it), otherwise as ti_launch does.
+template <typename... KArgs, typename... Args>
+cudaError_t ti_launch_clusters(void (*kernel)(KArgs...), dim3 grid, int ctas, dim3 block, cudaStream_t stream, Args... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = block;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = (unsigned)ctas;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = ti_pdl_enabled() ? 2 : 1;
+    return cudaLaunchKernelEx(&cfg, kernel, KArgs(args)...);
+}
+
 struct Best { float v; int i; };
 __device__ __forceinline__ Best better(Best a, Best b) {
     if (b.i < 0) return a;
