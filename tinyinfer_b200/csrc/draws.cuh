@@ -14,6 +14,10 @@ __device__ __forceinline__ uint4 philox4x32_10(uint4 c, uint2 k) {
     }
     return c;
 }
+__device__ __forceinline__ unsigned word_of(uint4 w, int i) {       // word i mod 4
+    const unsigned lo = (i & 1) ? w.y : w.x, hi = (i & 1) ? w.w : w.z;
+    return (i & 2) ? hi : lo;
+}
 __device__ __forceinline__ float philox_uniform(unsigned word) {   // in (0, 1), exact in float32
     return ((float)(word >> 9) + 0.5f) * (1.0f / 8388608.0f);
 }
@@ -22,12 +26,13 @@ __device__ __forceinline__ unsigned order_key(float v) {           // larger flo
     return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
 }
 
-// Launches `kernel` on clusters of `ctas` blocks along x (more than 8: the kernel has to allow it), otherwise as ti_launch does.
+// Launches `kernel` on clusters of `ctas` blocks along x, otherwise as ti_launch does.
 template <typename... KArgs, typename... Args>
-cudaError_t ti_launch_clusters(void (*kernel)(KArgs...), dim3 grid, int ctas, dim3 block, cudaStream_t stream, Args... args) {
+cudaError_t ti_launch_clusters(void (*kernel)(KArgs...), dim3 grid, int ctas, dim3 block, size_t smem, cudaStream_t stream, Args... args) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = grid;
     cfg.blockDim = block;
+    cfg.dynamicSmemBytes = smem;
     cfg.stream = stream;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;

@@ -14,8 +14,14 @@
 // Sums and exponentials are float32 (the sum over a top-k row's few candidates is taken in fixed point, so that the order in which
 // they were found does not show).
 //
-// Bound by reading the logits once: a row is held by a cluster of blocks, 40 logits a thread in registers (all its loads in flight at
-// once), so threshold, sum and draw take no second trip to memory. The blocks of a row meet in the first one's shared memory.
+// Bound by reading the logits once. Three kernels:
+//   parts_kernel   streams every row, 32 logits a thread in registers, and leaves of each warp's part the largest, the sum and the best
+//                  draw, or of a top-k row each THREAD's largest logit (a 32nd of the row); no block waits for another, no warp for another.
+//   topk_kernel    a block a top-k row: the k-th largest of 256 of these largest bounds the row's k-th largest from below, so the
+//                  row's top k are in the few threads' parts (some 130 for k = 100) that reach it; those are read again and ranked.
+//   verify_kernel  decides the request; behind a drawn draft that failed, clusters of blocks scan the two rows once more.
+// A row held by a cluster of 16 blocks in shared memory, threshold and sum found there, read the logits once too, but spent 13 us of a
+// block on meeting the others (a cluster's barrier 0.9 us) where its loads took 1.3: 291 us for 64 x 4 rows of 151,936 with k = 100.
 #include <cooperative_groups.h>
 
 #include "draws.cuh"
@@ -25,17 +31,20 @@ namespace cg = cooperative_groups;
 namespace {
 
 constexpr int VD_MAX_DRAFTS = 31;    // a warp decides a request: a lane a draft, and one place more
-constexpr int VD_THREADS = 512;
+constexpr int VD_THREADS = 256;
 constexpr int VD_WARPS = VD_THREADS / 32;
-constexpr int VD_GROUPS = 10;        // groups of four logits a thread holds
-constexpr int VD_SLICE = VD_THREADS * VD_GROUPS * 4;
-constexpr int VD_MAX_CTAS = 16;
-constexpr int VD_CANDIDATES = 2048;  // of a top-k row, in the first block's shared memory
+constexpr int VD_GROUPS = 8;         // groups of four logits a thread holds
+constexpr int VD_TILE = VD_THREADS * VD_GROUPS * 4;
+constexpr int VD_CANDIDATES = 4096;  // of a top-k row, in shared memory
+constexpr int VD_MAX_VOCAB = 1 << 19;        // so many weights of at most 2^44 fit 64 bits
 constexpr int VD_LIST = 256;         // of what the threshold keeps, for the draw behind a draft that failed
+constexpr int VD_CTAS = 8;           // blocks that share such a draw
 constexpr float LOG2E = 1.4426950408889634f;
 
-// What a row leaves: the largest scaled logit, the sum of the kept exponentials, the lowest kept key, the token that it draws (-1:
-// none; of a sampled row that a draft model's logits judge: not drawn yet), the share of its draft, how many kept tokens are listed.
+// A warp's part of a row: the largest scaled logit, the sum of the exponentials relative to it, the best draw.
+struct __align__(16) Part { float m, z, v; int i; };
+// A row: the largest scaled logit, the sum of the kept exponentials, the lowest kept key, the token that it draws (-1: none; of a
+// sampled row that a draft model's logits judge: not drawn), the share of its draft, how many kept tokens are listed (-1: not).
 struct __align__(16) RowStats { float m, z; unsigned threshold; int drawn; float share; int listed, unused[2]; };
 struct __align__(8) Kept { float s; int i; };
 
@@ -49,12 +58,14 @@ struct VdArgs {
     const int *stream_id, *step;
     const float* draft_logits;       // element (r, j, i) at r * draft_request + j * draft_place + i, or null
     long long draft_request, draft_place;
-    RowStats *target, *draft;        // [requests, max_drafts + 1], [requests, max_drafts]
+    float* parts;                    // [requests, places, tiles, VD_THREADS]: threads' largest logits, or warps' Parts
+    RowStats* stats;                 // [requests, places] of top-k rows
     Kept* kept;                      // [requests, max_drafts, VD_LIST]
     int* tokens;                     // [requests, max_drafts + 1]
     int* counts;
     float* accept;                   // [requests, max_drafts]
-    int rows, vocab, requests, max_drafts;
+    int rows, vocab, requests, max_drafts, tiles;
+    int places;                      // max_drafts + 1 rows of the target, then max_drafts of the draft model if there is one
 };
 
 // The request's rows: first flat row and how many (0 .. max_drafts + 1), inside the logits whatever cu_rows says.
@@ -66,6 +77,17 @@ __device__ __forceinline__ bool is_greedy(const VdArgs& a, int r) { return a.tem
 __device__ __forceinline__ uint2 seed_of(const VdArgs& a, int r) {
     return make_uint2((unsigned)(a.seed[r] & 0xFFFFFFFFll), (unsigned)((unsigned long long)a.seed[r] >> 32));
 }
+// A place of a request: which of its rows (-1: none) and where it lies. draws: its token is wanted whatever becomes of the drafts.
+struct Place { const float* x; int j; bool draws; };
+__device__ __forceinline__ Place place_of(const VdArgs& a, int r, int place, int2 rows, bool greedy) {
+    const bool of_draft = place > a.max_drafts;
+    const int j = of_draft ? place - a.max_drafts - 1 : place;
+    if (of_draft ? greedy || j >= rows.y - 1 : j >= rows.y) return Place{nullptr, -1, false};
+    const float* x = of_draft ? a.draft_logits + r * a.draft_request + j * a.draft_place : a.logits + (size_t)(rows.x + j) * a.vocab;
+    return Place{x, j, !greedy && !of_draft && (a.draft_logits == nullptr || j == rows.y - 1)};
+}
+__device__ __forceinline__ bool has_threshold(int topk, int vocab) { return topk > 0 && topk < vocab; }
+
 __device__ __forceinline__ unsigned score_key(float s) { return order_key(s + 0.f); }        // -0 and +0 are one value
 
 // The weights of a row's logits, exp(v / temp - m): 2^(v * c - m * log2 e), one multiply-add and one exponential. Where that has
@@ -76,34 +98,32 @@ struct Weights {
     __device__ __forceinline__ Weights(float temp_, float m_) : temp(temp_), m(m_), c(LOG2E / temp_), m2(m_ * LOG2E) {
         odd = !(fabsf(m) < 1e30f) || !(c < 1e30f);
     }
-    __device__ __forceinline__ float operator()(float v) const {
-        if (odd) {
-            const float s = v / temp;
-            return !(s > -INFINITY) ? 0.f : (s == m ? 1.f : expf(s - m));
-        }
-        return exp2f(fmaf(v, c, -m2));
+    __device__ __forceinline__ float fast(float v) const { return exp2f(fmaf(v, c, -m2)); }
+    __device__ __forceinline__ float quotient(float v) const {
+        const float s = v / temp;
+        return !(s > -INFINITY) ? 0.f : (s == m ? 1.f : expf(s - m));
     }
+    __device__ __forceinline__ float operator()(float v) const { return odd ? quotient(v) : fast(v); }
+    // A factor on the weights that covers what they and a score s + G are off by: 2^-24 of the scaled logits, several times over.
+    __device__ __forceinline__ float spare() const { return 1.001f + fabsf(m) * 1e-6f; }
 };
 // The same of a scaled logit at hand.
 __device__ __forceinline__ float scaled_weight(float s, float m) { return !(s > -INFINITY) ? 0.f : (s == m ? 1.f : exp2f((s - m) * LOG2E)); }
+
+// s + G of a scaled logit s and its uniform number.
+__device__ __forceinline__ float noisy(float s, float u) { return s - logf(-logf(u)); }
 
 __device__ __forceinline__ Best warp_best(Best v) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) v = better(v, Best{__shfl_xor_sync(~0u, v.v, o), __shfl_xor_sync(~0u, v.i, o)});
     return v;
 }
-__device__ __forceinline__ float warp_min(float v) {
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v = fminf(v, __shfl_xor_sync(~0u, v, o));
-    return v;
-}
-template <int WARPS>
 __device__ __forceinline__ Best block_best(Best x, Best* sh) {
     x = warp_best(x);
     __syncthreads();
     if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = x;
     __syncthreads();
-    return warp_best((threadIdx.x & 31) < WARPS ? sh[threadIdx.x & 31] : Best{0.f, -1});
+    return warp_best((threadIdx.x & 31) < VD_WARPS ? sh[threadIdx.x & 31] : Best{0.f, -1});
 }
 
 // A value that is below every logit whose quotient by temp reaches that of `bound`: quotients are rounded, by 2^-24 of themselves
@@ -113,329 +133,348 @@ __device__ __forceinline__ float below_quotient(float bound, float temp) {
     return s > 1e-35f && s < 1e37f ? bound - fabsf(bound) * 4.8e-7f : -INFINITY;
 }
 
-// A thread's part of a row, in groups of four logits: group (k * ctas + rank) * threads + tid. Which thread holds which logits goes by
-// their number alone, not by where the row lies, so that the order of sums does not either: a row off 16-byte boundaries (of an odd
-// vocabulary, say) is read 8 or 4 bytes at a time.
-struct Slice {
-    const float* x;                  // the row
-    int first, stride, vocab, step;
-    __device__ __forceinline__ Slice(const float* x_, int vocab_, int rank, int ctas)
-        : x(x_), first(4 * (rank * VD_THREADS + (int)threadIdx.x)), stride(4 * ctas * VD_THREADS), vocab(vocab_),
-          step(((uintptr_t)x_ & 15) == 0 ? 4 : ((uintptr_t)x_ & 7) == 0 ? 2 : 1) {}
-    __device__ __forceinline__ int token(int k) const { return first + k * stride; }        // the group's first
-    __device__ __forceinline__ void load(int k, float (&v)[4]) const {
-        const int e = token(k);
-        if (step == 4 && e + 3 < vocab) {
-            const float4 f = __ldcs(reinterpret_cast<const float4*>(x + e));
-            v[0] = f.x; v[1] = f.y; v[2] = f.z; v[3] = f.w;
-        } else if (step == 2 && e + 3 < vocab) {
-            const float2 f = *reinterpret_cast<const float2*>(x + e), g = *reinterpret_cast<const float2*>(x + e + 2);
-            v[0] = f.x; v[1] = f.y; v[2] = g.x; v[3] = g.y;
-        } else {                                         // also the row's end, and places behind it
+// Four neighbouring logits of a row; NaN behind its end. step: how many the row's place lets be read at once (rows off 16-byte
+// boundaries: of an odd vocabulary, say). Which thread reads which logits goes by their number alone, and so does the order of sums.
+__device__ __forceinline__ int row_step(const float* x) { return ((uintptr_t)x & 15) == 0 ? 4 : ((uintptr_t)x & 7) == 0 ? 2 : 1; }
+__device__ __forceinline__ void load_four(const float* x, int e, int vocab, int step, float (&v)[4]) {
+    if (step == 4 && e + 3 < vocab) {
+        const float4 f = *reinterpret_cast<const float4*>(x + e);
+        v[0] = f.x; v[1] = f.y; v[2] = f.z; v[3] = f.w;
+    } else if (step == 2 && e + 3 < vocab) {
+        const float2 f = *reinterpret_cast<const float2*>(x + e), g = *reinterpret_cast<const float2*>(x + e + 2);
+        v[0] = f.x; v[1] = f.y; v[2] = g.x; v[3] = g.y;
+    } else {
 #pragma unroll
-            for (int j = 0; j < 4; ++j) v[j] = e + j < vocab ? x[e + j] : NAN;
-        }
+        for (int j = 0; j < 4; ++j) v[j] = e + j < vocab ? x[e + j] : NAN;
     }
-};
-
-struct RowShared {
-    unsigned key[VD_CANDIDATES];
-    int idx[VD_CANDIDATES];
-    unsigned sums[4][256];           // the first block's: the row's histogram of each byte
-    unsigned hist[256], sel[2];
-    float bound[VD_MAX_CTAS], m[VD_MAX_CTAS], z[VD_MAX_CTAS];
-    Best part[VD_MAX_CTAS];
-    float warp[VD_WARPS], red[33];
-    Best best[VD_WARPS];
-    unsigned long long total[VD_WARPS];
-    int count, over, listed;
-};
-
-// The k-th largest key of the row by radix selection over what the blocks hold, all blocks together; any k, any number of ties.
-__device__ __forceinline__ unsigned row_threshold(RowShared& sh, cg::cluster_group& cluster, const float (&v)[VD_GROUPS][4], const Slice& s, float temp, int k) {
-    const int tid = threadIdx.x;
-    unsigned prefix = 0u, left = (unsigned)k;
-    for (int pass = 0; pass < 4; ++pass) {
-        const int shift = 24 - 8 * pass;
-        const unsigned mask = pass == 0 ? 0u : 0xFFFFFFFFu << (shift + 8);
-        if (tid < 256) sh.hist[tid] = 0u;
-        __syncthreads();
-#pragma unroll
-        for (int g = 0; g < VD_GROUPS; ++g) {
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const unsigned key = score_key(v[g][j] / temp);
-                if (v[g][j] > -INFINITY && (key & mask) == prefix) {
-                    const unsigned bin = (key >> shift) & 0xFFu, same = __match_any_sync(__activemask(), bin);
-                    if ((tid & 31) == __ffs(same) - 1) atomicAdd(&sh.hist[bin], (unsigned)__popc(same));
-                }
-            }
-        }
-        __syncthreads();
-        if (tid < 256 && sh.hist[tid]) atomicAdd(cluster.map_shared_rank(&sh.sums[pass][tid], 0), sh.hist[tid]);
-        cluster.sync();
-        if (cluster.block_rank() == 0 && tid < 32) {         // a lane eight bins; the highest whose bins, with all above, reach the k-th
-            unsigned mine[8], sum = 0u;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) { mine[i] = sh.sums[pass][8 * tid + i]; sum += mine[i]; }
-            unsigned above = sum;
-#pragma unroll
-            for (int off = 1; off < 32; off <<= 1) {
-                const unsigned w = __shfl_down_sync(~0u, above, off);
-                if (tid + off < 32) above += w;
-            }
-            const unsigned reach = __ballot_sync(~0u, above >= left);
-            if (reach ? tid == 31 - __clz(reach) : tid == 0) {
-                unsigned want = left - (above - sum);
-                int b = 7;
-                if (reach) {
-                    for (; b > 0 && mine[b] < want; --b) want -= mine[b];
-                } else {                                     // fewer than k: all of them
-                    b = 0;
-                    want = 0u;
-                }
-                sh.sel[0] = reach ? prefix | ((unsigned)(8 * tid + b) << shift) : 0u;
-                sh.sel[1] = want;
-            }
-        }
-        cluster.sync();
-        prefix = *cluster.map_shared_rank(&sh.sel[0], 0);
-        left = *cluster.map_shared_rank(&sh.sel[1], 0);
-        if (left == 0u) break;
-    }
-    cluster.sync();                                          // the first block goes on only when all have read
-    return left == 0u ? 0u : prefix;
 }
 
-__global__ void __launch_bounds__(VD_THREADS, 2) row_kernel(VdArgs a) {
-    __shared__ RowShared sh;
-    cg::cluster_group cluster = cg::this_cluster();
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, rank = blockIdx.x, ctas = gridDim.x;
-    const int r = blockIdx.z, place = blockIdx.y, D = a.max_drafts;
+// The tokens of thread t in a tile: groups of four, VD_THREADS groups apart.
+__device__ __forceinline__ int token_of(int tile, int t, int k) { return tile * VD_TILE + 4 * (t + k * VD_THREADS); }
+
+__global__ void __launch_bounds__(VD_THREADS, 4) parts_kernel(VdArgs a) {
     ti_grid_launch_dependents();
     ti_grid_wait();
+    const int tid = threadIdx.x, lane = tid & 31, r = blockIdx.z;
     const int2 rows = rows_of(a, r);
-    const bool greedy = is_greedy(a, r), of_draft = place > D;
-    const int j = of_draft ? place - D - 1 : place;
-    if (of_draft ? greedy || j >= rows.y - 1 : j >= rows.y) return;
-    const float* x = of_draft ? a.draft_logits + r * a.draft_request + j * a.draft_place : a.logits + (size_t)(rows.x + j) * a.vocab;
-    const Slice slice(x, a.vocab, rank, ctas);
+    const bool greedy = is_greedy(a, r);
+    const Place at = place_of(a, r, blockIdx.y, rows, greedy);
+    if (at.j < 0) return;
+    const int step = row_step(at.x);
     float v[VD_GROUPS][4];
+    if (step == 4 && token_of(blockIdx.x + 1, 0, 0) <= a.vocab) {
+        const float4* from = reinterpret_cast<const float4*>(at.x + token_of(blockIdx.x, tid, 0));
 #pragma unroll
-    for (int k = 0; k < VD_GROUPS; ++k) slice.load(k, v[k]);
-    const int drafted = j < rows.y - 1 ? a.token_ids[rows.x + j + 1] : -1;
-    const float at_draft = drafted >= 0 && drafted < a.vocab ? x[drafted] : NAN;
-    const float temp = greedy ? 1.f : a.temperature[r];
-    const int topk = greedy ? 0 : a.topk[r];
-    const bool draws = !greedy && !of_draft && (a.draft_logits == nullptr || j == rows.y - 1);
-    const uint2 key2 = draws ? seed_of(a, r) : make_uint2(0u, 0u);
-    const unsigned c1 = draws ? (unsigned)(a.step[r] + j) : 0u, stream = draws ? (unsigned)a.stream_id[r] : 0u;
-    // what the other blocks write to or count in
-    if (tid < 256)
-        for (int p = 0; p < 4; ++p) sh.sums[p][tid] = 0u;
-    if (tid == 0) sh.count = sh.over = sh.listed = 0;
-    cluster.sync();
-    RowStats* out = of_draft ? a.draft + r * D + j : a.target + r * (D + 1) + j;
-    RowStats st{0.f, 0.f, 0u, -1, 0.f, -1, {0, 0}};
+        for (int k = 0; k < VD_GROUPS; ++k) {
+            const float4 f = from[k * VD_THREADS];
+            v[k][0] = f.x; v[k][1] = f.y; v[k][2] = f.z; v[k][3] = f.w;
+        }
+    } else {
+#pragma unroll
+        for (int k = 0; k < VD_GROUPS; ++k) load_four(at.x, token_of(blockIdx.x, tid, k), a.vocab, step, v[k]);
+    }
+    float* out = a.parts + (((size_t)r * a.places + blockIdx.y) * a.tiles + blockIdx.x) * VD_THREADS;
+    Part* part = reinterpret_cast<Part*>(out) + (tid >> 5);
 
     if (greedy) {
         Best b{-INFINITY, -1};
 #pragma unroll
-        for (int k = 0; k < VD_GROUPS; ++k) {
+        for (int k = 0; k < VD_GROUPS; ++k)
 #pragma unroll
             for (int q = 0; q < 4; ++q)                      // a thread's tokens come in their order: the first of equals stays
-                if (v[k][q] > b.v || (b.i < 0 && v[k][q] == v[k][q])) b = Best{v[k][q], slice.token(k) + q};
-        }
-        b = block_best<VD_WARPS>(b, sh.best);
-        if (tid == 0) *cluster.map_shared_rank(&sh.part[rank], 0) = b;
-        cluster.sync();
-        if (rank == 0 && warp == 0) {
-            b = warp_best(lane < ctas ? sh.part[lane] : Best{0.f, -1});
-            st.drawn = b.i;
-            if (lane == 0) *out = st;
-        }
+                if (v[k][q] > b.v || (b.i < 0 && v[k][q] == v[k][q])) b = Best{v[k][q], token_of(blockIdx.x, tid, k) + q};
+        b = warp_best(b);
+        if (lane == 0) *part = Part{0.f, 0.f, b.v, b.i};
         return;
     }
-
     float most = -INFINITY;
 #pragma unroll
-    for (int k = 0; k < VD_GROUPS; ++k) {
+    for (int k = 0; k < VD_GROUPS; ++k)
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
-            v[k][q] = fmaxf(v[k][q], -INFINITY);             // NaN and places outside the row: -inf
+            v[k][q] = fmaxf(v[k][q], -INFINITY);             // NaN, and what lies behind the row: -inf
             most = fmaxf(most, v[k][q]);
         }
+    if (has_threshold(a.topk[r], a.vocab)) {
+        out[tid] = most;
+        return;
     }
-    if (topk > 0 && topk < a.vocab) {
-        bool wide = topk > ctas * VD_THREADS;                // more than there are threads to offer a value each
-        if (!wide) {
-            // Every warp offers the u-th largest of its threads' largest logits, u * warps >= k: at least k logits of the row
-            // reach the least of these offers, and few more do. Those are the row's candidates.
-            const int u = (topk + ctas * VD_WARPS - 1) / (ctas * VD_WARPS);
-            float offer = 0.f, rest = most;
-            for (int i = 0; i < u; ++i) {
-                offer = warp_max(rest);
-                const unsigned who = __ballot_sync(~0u, rest == offer);
-                if (lane == __ffs(who) - 1) rest = -INFINITY;
+    const float temp = a.temperature[r], m = warp_max(most) / temp;
+    const Weights weight(temp, m);
+    float z = 0.f;
+    if (weight.odd) {
+        if (m > -INFINITY) {
+#pragma unroll 1
+            for (int i = 0; i < 4 * VD_GROUPS; ++i) {
+                const int e = token_of(blockIdx.x, tid, i >> 2) + (i & 3);
+                if (e < a.vocab) z += weight.quotient(at.x[e]);
             }
-            if (lane == 0) sh.warp[warp] = offer;
-            __syncthreads();
-            const float least = warp_min(lane < VD_WARPS ? sh.warp[lane] : INFINITY);
-            if (tid < ctas) *cluster.map_shared_rank(&sh.bound[rank], tid) = least;
-            cluster.sync();
-            const float low = below_quotient(warp_min(lane < ctas ? sh.bound[lane] : INFINITY), temp);
-            int n = 0;
-            if (most >= low && most > -INFINITY) {
+        }
+    } else {                                                 // from here on v is the weight
 #pragma unroll
-                for (int k = 0; k < VD_GROUPS; ++k) {
+        for (int k = 0; k < VD_GROUPS; ++k) {
 #pragma unroll
-                    for (int q = 0; q < 4; ++q) n += v[k][q] >= low && v[k][q] > -INFINITY;
-                }
-            }
-            int before = n;
+            for (int q = 0; q < 4; ++q) v[k][q] = weight.fast(v[k][q]);
+            z += (v[k][0] + v[k][1]) + (v[k][2] + v[k][3]);
+        }
+        most = weight.fast(most);
+    }
+    z = warp_sum(z);
+    Best b{-INFINITY, -1};
+    if (at.draws && m > -INFINITY) {
+        // The largest of s + G, G = -log E, E = -log U. A token can pass a score B only if E < exp(s - B); E is 1 - U at least, and 1 - U
+        // is exact: one comparison settles all but a few tokens once some B is known.
+        const uint2 key2 = seed_of(a, r);
+        const unsigned c1 = (unsigned)(a.step[r] + at.j), stream = (unsigned)a.stream_id[r];
+        float spare = 0.f;                                   // exp(m - B)
+#pragma unroll 1
+        for (int half = 0; half < 2; ++half) {               // the threads' largest logits for a first B, then all
+            unsigned left = 0u;
 #pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const int w = __shfl_up_sync(~0u, before, o);
-                if (lane >= o) before += w;
-            }
-            int base = 0;
-            if (lane == 31 && before > 0) {
-                base = atomicAdd(cluster.map_shared_rank(&sh.count, 0), before);
-                if (base + before > VD_CANDIDATES)
-                    for (int c = 0; c < ctas; ++c) *cluster.map_shared_rank(&sh.over, c) = 1;
-            }
-            int at = __shfl_sync(~0u, base, 31) + before - n;
-            if (n > 0) {
-                unsigned* keys = cluster.map_shared_rank(sh.key, 0);
-                int* idx = cluster.map_shared_rank(sh.idx, 0);
+            for (int k = 0; k < VD_GROUPS; ++k) {
+                if (half == 0) {
 #pragma unroll
-                for (int k = 0; k < VD_GROUPS; ++k) {
+                    for (int q = 0; q < 4; ++q) left = v[k][q] == most ? 1u << (4 * k + q) : left;
+                } else {
+                    const uint4 w = philox4x32_10(make_uint4((unsigned)token_of(blockIdx.x, tid, k) >> 2, c1, stream, 0u), key2);
+                    const unsigned words[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
                     for (int q = 0; q < 4; ++q)
-                        if (v[k][q] >= low && v[k][q] > -INFINITY) {
-                            if (at < VD_CANDIDATES) { keys[at] = score_key(v[k][q] / temp); idx[at] = slice.token(k) + q; }
-                            ++at;
-                        }
+                        left |= (weight.odd ? v[k][q] > -INFINITY : 1.f - philox_uniform(words[q]) < v[k][q] * spare) ? 1u << (4 * k + q) : 0u;
                 }
             }
-            cluster.sync();
-            wide = sh.over != 0;
+            if (half == 0 && !(most > (weight.odd ? -INFINITY : 0.f))) left = 0u;       // (a weight of nothing is beaten by the largest)
+            for (; left; left &= left - 1u) {                // (their numbers once more: the register file has no subscripts)
+                const int bit = __ffs(left) - 1, i = token_of(blockIdx.x, tid, bit >> 2) + (bit & 3);
+                const uint4 w = philox4x32_10(make_uint4((unsigned)i >> 2, c1, stream, 0u), key2);
+                b = better(b, Best{noisy(at.x[i] / temp, philox_uniform(word_of(w, i))), i});
+            }
+            if (!weight.odd) spare = exp2f((m - warp_max(b.v)) * LOG2E) * weight.spare();
         }
-        if (!wide) {
-            if (rank != 0) return;
-            // the first block alone, on the candidates
-            const int n = sh.count;
-            if (n > topk)
+        b = warp_best(b);
+    }
+    if (lane == 0) *part = Part{m, z, b.v, b.i};
+}
+
+struct TopShared {
+    alignas(16) float most[VD_THREADS];                       // read four at a time
+    unsigned key[VD_CANDIDATES];
+    int idx[VD_CANDIDATES];          // of the candidates; before them, the threads' parts that hold some
+    unsigned hist[256], sel[2];
+    float red[33];
+    Best best[VD_WARPS];
+    unsigned long long total[VD_WARPS];
+    float bound;
+    int parts, count, listed;
+};
+
+// A value that at least k of the threads' largest logits reach; -inf if there is none.
+__device__ __forceinline__ float top_bound(TopShared& sh, const float* largest, int n, int k) {
+    const int tid = threadIdx.x;
+    if (k > n) return -INFINITY;
+    if (k <= VD_THREADS) {
+        // every thread takes the largest of its share of them; the k-th largest of these 256, found by counting
+        float own = -INFINITY;
+        for (int i = tid; i < n; i += VD_THREADS) own = fmaxf(own, largest[i]);
+        sh.most[tid] = own;
+        __syncthreads();
+        int above = 0, level = 0;
+        const float4* most = reinterpret_cast<const float4*>(sh.most);
+#pragma unroll 8
+        for (int i = 0; i < VD_THREADS / 4; ++i) {
+            const float4 o = most[i];
+            above += (o.x > own) + (o.y > own) + (o.z > own) + (o.w > own);
+            level += (o.x == own) + (o.y == own) + (o.z == own) + (o.w == own);
+        }
+        if (above < k && k <= above + level) sh.bound = own;         // the same value from each that finds it
+        __syncthreads();
+        return sh.bound;
+    }
+    unsigned lo = order_key(-INFINITY), hi = order_key(INFINITY);     // at least k reach lo
+    for (int i = 0; i < 20 && lo < hi; ++i) {
+        const unsigned middle = lo + (hi - lo + 1) / 2;
+        int reach = 0;
+        for (int j = tid; j < n; j += VD_THREADS) reach += order_key(largest[j]) >= middle;
+        reach = (int)block_sum((float)reach, sh.red);                 // at most 2^24 of them: exact
+        if (reach >= k) lo = middle;
+        else hi = middle - 1;
+    }
+    return key_value(lo);
+}
+
+__global__ void __launch_bounds__(VD_THREADS) topk_kernel(VdArgs a) {
+    __shared__ TopShared sh;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, r = blockIdx.y, D = a.max_drafts;
+    ti_grid_launch_dependents();
+    if (tid == 0) sh.parts = sh.count = sh.listed = 0;
+    __syncthreads();
+    ti_grid_wait();
+    const int2 rows = rows_of(a, r);
+    const bool greedy = is_greedy(a, r);
+    const Place at = place_of(a, r, blockIdx.x, rows, greedy);
+    const int topk = greedy ? 0 : a.topk[r];
+    if (at.j < 0 || !has_threshold(topk, a.vocab)) return;
+    const float temp = a.temperature[r];
+    const int drafted = at.j < rows.y - 1 ? a.token_ids[rows.x + at.j + 1] : -1;
+    const float at_draft = drafted >= 0 && drafted < a.vocab ? at.x[drafted] : NAN;
+    const uint2 key2 = at.draws ? seed_of(a, r) : make_uint2(0u, 0u);
+    const unsigned c1 = at.draws ? (unsigned)(a.step[r] + at.j) : 0u, stream = at.draws ? (unsigned)a.stream_id[r] : 0u;
+    const size_t slot = (size_t)r * a.places + blockIdx.x;
+    const float* largest = a.parts + slot * a.tiles * VD_THREADS;
+    const int n_largest = a.tiles * VD_THREADS, step = row_step(at.x);
+    const bool lists = !at.draws && (int)blockIdx.x <= D;             // a draw behind a failed draft may want them
+    Kept* kept = lists ? a.kept + ((size_t)r * D + at.j) * VD_LIST : nullptr;
+    RowStats st{0.f, 0.f, 0u, -1, 0.f, -1, {0, 0}};
+    unsigned long long sum = 0;                                       // weights of at most 1 in steps of 2^-44
+    Best b{0.f, -1};
+
+    const float low = below_quotient(top_bound(sh, largest, n_largest, topk), temp);
+    for (int i = tid; i < n_largest; i += VD_THREADS) {
+        const float v = largest[i];
+        if (v >= low && v > -INFINITY) {
+            const int to = atomicAdd(&sh.parts, 1);
+            if (to < VD_CANDIDATES) sh.idx[to] = i;
+        }
+    }
+    __syncthreads();
+    const int n_parts = sh.parts;
+    bool fits = n_parts <= VD_CANDIDATES;
+    if (fits) {
+        // their logits once more, a thread a group; what reaches the bound takes the places behind them and is moved when all is found
+        for (int first = 0; first < n_parts * VD_GROUPS; first += VD_THREADS) {
+            const int w = first + tid;
+            float v[4] = {NAN, NAN, NAN, NAN};
+            int e = 0;
+            if (w < n_parts * VD_GROUPS) {
+                const int i = sh.idx[w / VD_GROUPS];
+                e = token_of(i / VD_THREADS, i % VD_THREADS, w % VD_GROUPS);
+                load_four(at.x, e, a.vocab, step, v);
+            }
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+                if (v[q] >= low && v[q] > -INFINITY) {
+                    const int to = atomicAdd(&sh.count, 1);
+                    if (to < VD_CANDIDATES) sh.key[to] = (unsigned)(e + q);
+                }
+        }
+        __syncthreads();
+        fits = sh.count <= VD_CANDIDATES;
+    }
+    if (fits) {
+        const int n = sh.count;
+        for (int i = tid; i < n; i += VD_THREADS) {
+            const int token = (int)sh.key[i];
+            sh.idx[i] = token;
+            sh.key[i] = score_key(at.x[token] / temp);
+        }
+        __syncthreads();
+        if (n >= topk) {                                              // fewer: no finite logit of the row is missing, and all are kept
+            if (n <= 2 * VD_THREADS) {
+                // the k-th largest is the key that fewer than k pass and with its equals k reach
+                for (int i = tid; i < n; i += VD_THREADS) {
+                    const unsigned own = sh.key[i];
+                    int above = 0, level = 0;
+                    for (int o = 0; o < n; ++o) { above += sh.key[o] > own; level += sh.key[o] == own; }
+                    if (above < topk && topk <= above + level) sh.sel[0] = own;
+                }
+                __syncthreads();
+                st.threshold = sh.sel[0];
+            } else {
                 st.threshold = select_kth(topk, sh.hist, sh.sel, [&](auto count) {
                     for (int i = tid; i < n; i += VD_THREADS) count(sh.key[i]);
                 });
-            unsigned top = 0u;
-            for (int i = tid; i < n; i += VD_THREADS) top = max(top, sh.key[i]);
-            top = __reduce_max_sync(~0u, top);
-            if (lane == 0) sh.warp[warp] = __uint_as_float(top);
-            __syncthreads();
-            top = __reduce_max_sync(~0u, lane < VD_WARPS ? __float_as_uint(sh.warp[lane]) : 0u);
-            st.m = n > 0 ? key_value(top) : -INFINITY;
-            unsigned long long sum = 0;                      // weights of at most 1 in steps of 2^-44
-            Best b{0.f, -1};
-            const bool lists = !draws && !of_draft;
-            for (int i = tid; i < n; i += VD_THREADS) {
-                if (sh.key[i] < st.threshold) continue;
-                const float s = key_value(sh.key[i]);
-                sum += __float2ull_rn(scaled_weight(s, st.m) * 17592186044416.f);
-                if (draws) {
-                    const uint4 w = philox4x32_10(make_uint4((unsigned)sh.idx[i] >> 2, c1, stream, 0u), key2);
-                    const unsigned words[4] = {w.x, w.y, w.z, w.w};
-                    b = better(b, Best{s - logf(-logf(philox_uniform(words[sh.idx[i] & 3]))), sh.idx[i]});
-                }
-                if (lists) {
-                    const int slot = atomicAdd(&sh.listed, 1);
-                    if (slot < VD_LIST) a.kept[((size_t)r * D + j) * VD_LIST + slot] = Kept{s, sh.idx[i]};
-                }
             }
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
-            if (lane == 0) sh.total[warp] = sum;
-            b = block_best<VD_WARPS>(b, sh.best);
-            if (tid == 0) {
-                sum = 0;
-                for (int w = 0; w < VD_WARPS; ++w) sum += sh.total[w];
-                st.z = (float)((double)sum * (1.0 / 17592186044416.0));
-                st.drawn = b.i;
-                const float s = at_draft / temp;
-                if (s > -INFINITY && score_key(s) >= st.threshold) st.share = scaled_weight(s, st.m) / st.z;
-                if (lists && sh.listed <= VD_LIST) st.listed = sh.listed;
-                *out = st;
+        }
+        unsigned top = 0u;
+        for (int i = tid; i < n; i += VD_THREADS) top = max(top, sh.key[i]);
+        top = __reduce_max_sync(~0u, top);
+        if (lane == 0) sh.most[warp] = __uint_as_float(top);
+        __syncthreads();
+        top = __reduce_max_sync(~0u, lane < VD_WARPS ? __float_as_uint(sh.most[lane]) : 0u);
+        st.m = n > 0 ? key_value(top) : -INFINITY;
+        for (int i = tid; i < n; i += VD_THREADS) {
+            if (sh.key[i] < st.threshold) continue;
+            const float s = key_value(sh.key[i]);
+            sum += __float2ull_rn(scaled_weight(s, st.m) * 17592186044416.f);
+            if (at.draws) {
+                const uint4 w = philox4x32_10(make_uint4((unsigned)sh.idx[i] >> 2, c1, stream, 0u), key2);
+                b = better(b, Best{noisy(s, philox_uniform(word_of(w, sh.idx[i]))), sh.idx[i]});
             }
-            return;
-        }
-        st.threshold = row_threshold(sh, cluster, v, slice, temp, topk);
-    }
-
-    // Every kept logit of the row counts: the blocks' sums and best draws, each relative to its own largest.
-    most = warp_max(most);
-    if (lane == 0) sh.warp[warp] = most;
-    __syncthreads();
-    const float m = warp_max(lane < VD_WARPS ? sh.warp[lane] : -INFINITY) / temp;
-    const Weights weight(temp, m);
-    const unsigned threshold = st.threshold;
-    float z = 0.f;
-#pragma unroll
-    for (int k = 0; k < VD_GROUPS; ++k) {
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            if (threshold && score_key(v[k][q] / temp) < threshold) v[k][q] = -INFINITY;
-            if (v[k][q] > -INFINITY) z += weight(v[k][q]);
-        }
-    }
-    z = block_sum(z, sh.red);
-    Best b{-INFINITY, -1};
-    if (draws) {
-        // The largest of s + G, G = -log E, E = -log U. A token can pass the best score B so far only if E < exp(s - B), that is, since
-        // exp(-y) >= 1 - y, if U > 1 - exp(s - B): one comparison (with a thousandth to spare) settles all but a few tokens.
-        float spare = INFINITY;                              // exp(m - B)
-#pragma unroll
-        for (int k = 0; k < VD_GROUPS; ++k) {
-            const int e = slice.token(k);
-            if (e < a.vocab) {
-                const uint4 w = philox4x32_10(make_uint4((unsigned)e >> 2, c1, stream, 0u), key2);
-                const unsigned words[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    const float u = philox_uniform(words[q]);
-                    if (v[k][q] > -INFINITY && !(u <= 1.f - weight(v[k][q]) * spare)) b = better(b, Best{v[k][q] / temp - logf(-logf(u)), e + q});
-                }
+            if (lists) {
+                const int to = atomicAdd(&sh.listed, 1);
+                if (to < VD_LIST) kept[to] = Kept{s, sh.idx[i]};
             }
-            if (k == 0 || k == 1 || k == 3) spare = exp2f((m - warp_max(b.v)) * LOG2E) * 1.001f;
         }
-        b = block_best<VD_WARPS>(b, sh.best);
+    } else {
+        // More candidates than there is room for (a k in the thousands, thousands of equal logits): the row itself, pass by pass.
+        st.threshold = select_kth(topk, sh.hist, sh.sel, [&](auto count) {
+            for (int i = tid; i < a.vocab; i += VD_THREADS) {
+                const float s = at.x[i] / temp;
+                if (s == s) count(score_key(s));
+            }
+        });
+        float top = -INFINITY;
+        for (int i = tid; i < a.vocab; i += VD_THREADS) top = fmaxf(top, at.x[i] / temp);
+        st.m = block_max(top, sh.red);
+        for (int i = tid; i < a.vocab; i += VD_THREADS) {
+            const float s = at.x[i] / temp;
+            if (!(s > -INFINITY) || score_key(s) < st.threshold) continue;
+            sum += __float2ull_rn(scaled_weight(s, st.m) * 17592186044416.f);
+            if (at.draws) {
+                const uint4 w = philox4x32_10(make_uint4((unsigned)i >> 2, c1, stream, 0u), key2);
+                b = better(b, Best{noisy(s, philox_uniform(word_of(w, i))), i});
+            }
+        }
+        if (tid == 0) sh.listed = VD_LIST + 1;
     }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
+    if (lane == 0) sh.total[warp] = sum;
+    b = block_best(b, sh.best);
     if (tid == 0) {
-        *cluster.map_shared_rank(&sh.m[rank], 0) = m;
-        *cluster.map_shared_rank(&sh.z[rank], 0) = z;
-        *cluster.map_shared_rank(&sh.part[rank], 0) = b;
-    }
-    cluster.sync();
-    if (rank == 0 && warp == 0) {
-        b = warp_best(lane < ctas ? sh.part[lane] : Best{0.f, -1});
-        const float mine = lane < ctas ? sh.m[lane] : -INFINITY;
-        st.m = warp_max(mine);
-        st.z = warp_sum(lane < ctas && sh.z[lane] > 0.f ? sh.z[lane] * scaled_weight(mine, st.m) : 0.f);
-        st.drawn = draws ? b.i : -1;
+        sum = 0;
+        for (int w = 0; w < VD_WARPS; ++w) sum += sh.total[w];
+        st.z = (float)((double)sum * (1.0 / 17592186044416.0));
+        st.drawn = b.i;
         const float s = at_draft / temp;
-        if (s > -INFINITY && score_key(s) >= threshold) st.share = Weights(temp, st.m)(at_draft) / st.z;
-        if (lane == 0) *out = st;
+        if (s > -INFINITY && score_key(s) >= st.threshold) st.share = scaled_weight(s, st.m) / st.z;
+        if (lists && sh.listed <= VD_LIST) st.listed = sh.listed;
+        a.stats[slot] = st;
     }
 }
 
-// Decides the request by its rows; if a drawn draft failed, draws from what is left of p beyond q. JUDGED: clusters of blocks share that
-// draw's row out; otherwise a warp a request.
-constexpr int VF_THREADS = 256;
-constexpr int VF_CTAS = 8;
+// What a warp's parts of a row come to: all of it for the row's warp.
+__device__ __forceinline__ RowStats whole_row(const VdArgs& a, const Place& at, size_t slot, bool greedy, float temp, int drafted) {
+    const int lane = threadIdx.x & 31, n = a.tiles * VD_WARPS;
+    const Part* part = reinterpret_cast<const Part*>(a.parts + slot * a.tiles * VD_THREADS);
+    auto nth = [&](int i) { return part[(i / VD_WARPS) * (VD_THREADS / 4) + i % VD_WARPS]; };
+    RowStats st{-INFINITY, 0.f, 0u, -1, 0.f, -1, {0, 0}};
+    const float at_draft = !greedy && drafted >= 0 && drafted < a.vocab ? at.x[drafted] : NAN;
+    Best b{0.f, -1};
+    float z = 0.f;
+    for (int i = lane; i < n; i += 32) {
+        const Part p = nth(i);
+        b = better(b, Best{p.v, p.i});
+        if (!greedy && p.z > 0.f) {
+            if (p.m > st.m) { z *= scaled_weight(st.m, p.m); st.m = p.m; }
+            z += p.z * scaled_weight(p.m, st.m);
+        }
+    }
+    st.drawn = warp_best(b).i;
+    if (greedy) return st;
+    const float m = warp_max(st.m);
+    st.z = warp_sum(z > 0.f ? z * scaled_weight(st.m, m) : 0.f);
+    st.m = m;
+    if (at_draft > -INFINITY) st.share = Weights(temp, m)(at_draft) / st.z;
+    return st;
+}
 
+// Decides the request by its rows; if a drawn draft failed, draws from what is left of p beyond q. JUDGED: a cluster of blocks a
+// request, which share that draw's rows out; otherwise a block.
 template <bool JUDGED>
-__global__ void __launch_bounds__(JUDGED ? VF_THREADS : 32) verify_kernel(VdArgs a) {
-    __shared__ Best best_sh[VF_THREADS / 32], part_sh[VF_CTAS];
+__global__ void __launch_bounds__(VD_THREADS) verify_kernel(VdArgs a) {
+    __shared__ RowStats row_sh[2 * VD_MAX_DRAFTS + 1];
+    __shared__ Best best_sh[VD_WARPS], part_sh[VD_CTAS];
     __shared__ int held_sh;
     ti_grid_launch_dependents();
     ti_grid_wait();
@@ -445,20 +484,29 @@ __global__ void __launch_bounds__(JUDGED ? VF_THREADS : 32) verify_kernel(VdArgs
     const bool greedy = is_greedy(a, r);
     const int n = rows.y - 1;
     const bool judged = JUDGED && !greedy;                   // by the ratio of the probabilities
+    const float temp = greedy ? 1.f : a.temperature[r];
+    const bool thresholded = !greedy && has_threshold(a.topk[r], a.vocab);
     const uint2 key2 = judged ? seed_of(a, r) : make_uint2(0u, 0u);
     const unsigned step = judged ? (unsigned)a.step[r] : 0u, stream = judged ? (unsigned)a.stream_id[r] : 0u;
-    int fed = -1;                                            // lane j: the draft j
+    const int fed = tid < n ? a.token_ids[rows.x + tid + 1] : -1;     // the draft of lane tid
+    for (int place = tid >> 5; place < a.places; place += VD_WARPS) {
+        const Place at = place_of(a, r, place, rows, greedy);
+        if (at.j < 0) continue;
+        const size_t slot = (size_t)r * a.places + place;
+        const RowStats st = thresholded ? a.stats[slot]
+                                        : whole_row(a, at, slot, greedy, temp, at.j < n ? a.token_ids[rows.x + at.j + 1] : -1);
+        if ((tid & 31) == 0) row_sh[place] = st;
+    }
+    __syncthreads();
     if (tid < 32) {
         bool holds = false;
         if (tid < D) {
             float prob = 0.f;
             if (tid < n) {
-                fed = a.token_ids[rows.x + tid + 1];
-                const RowStats st = a.target[r * (D + 1) + tid];
-                holds = fed >= 0 && fed == st.drawn;
-                prob = greedy ? (holds ? 1.f : 0.f) : st.share;
+                holds = fed >= 0 && fed == row_sh[tid].drawn;
+                prob = greedy ? (holds ? 1.f : 0.f) : row_sh[tid].share;
                 if (judged) {
-                    const float q = a.draft[r * D + tid].share;
+                    const float q = row_sh[D + 1 + tid].share;
                     prob = q > 0.f ? fminf(prob / q, 1.f) : (prob > 0.f ? 1.f : 0.f);
                     holds = philox_uniform(philox4x32_10(make_uint4(0u, step + tid, stream, 1u), key2).x) < prob;
                 }
@@ -472,12 +520,11 @@ __global__ void __launch_bounds__(JUDGED ? VF_THREADS : 32) verify_kernel(VdArgs
     const int held = held_sh;
     Best b{0.f, -1};
     if (rows.y > 0) {
-        const RowStats st = a.target[r * (D + 1) + held];
+        const RowStats st = row_sh[held];
         b.i = st.drawn;
         if (JUDGED && judged && held < n) {
             const unsigned c1 = step + held;
-            const RowStats ds = a.draft[r * D + held];
-            const float temp = a.temperature[r];
+            const RowStats ds = row_sh[D + 1 + held];
             const float* x = a.logits + (size_t)(rows.x + held) * a.vocab;
             const float* y = a.draft_logits + r * a.draft_request + held * a.draft_place;
             const Weights pw(temp, st.m), qw(temp, ds.m);
@@ -488,28 +535,51 @@ __global__ void __launch_bounds__(JUDGED ? VF_THREADS : 32) verify_kernel(VdArgs
             auto race = [&](float share, int i) {
                 if (!(share > 0.f)) return;
                 const uint4 w = philox4x32_10(make_uint4((unsigned)i >> 2, c1, stream, 2u), key2);
-                const unsigned words[4] = {w.x, w.y, w.z, w.w};
-                b = better(b, Best{share / -logf(philox_uniform(words[i & 3])), i});
+                b = better(b, Best{share / -logf(philox_uniform(word_of(w, i))), i});
             };
             b.i = -1;
             if (st.listed >= 0) {                            // the threshold keeps few: the first block alone
                 if (rank != 0) return;
                 const Kept* list = a.kept + ((size_t)r * D + held) * VD_LIST;
-                for (int i = tid; i < st.listed; i += VF_THREADS) race(scaled_weight(list[i].s, st.m) * pz - q_of(y[list[i].i]), list[i].i);
-                b = block_best<VF_THREADS / 32>(b, best_sh);
+                for (int i = tid; i < st.listed; i += VD_THREADS) race(scaled_weight(list[i].s, st.m) * pz - q_of(y[list[i].i]), list[i].i);
+                b = block_best(b, best_sh);
             } else {
+                // Only tokens whose share can still pass the best B of the warp run: share / E > B needs 1 - U < share / B.
                 cg::cluster_group cluster = cg::this_cluster();
-                for (int i = rank * VF_THREADS + tid; i < a.vocab; i += VF_CTAS * VF_THREADS) race(p_of(x[i]) - q_of(y[i]), i);
-                b = block_best<VF_THREADS / 32>(b, best_sh);
+                const int groups = (a.vocab + 3) / 4, x_step = row_step(x), y_step = row_step(y);
+                float spare = INFINITY;                      // 1 / B
+                for (int first = rank * VD_THREADS; first < groups; first += VD_CTAS * VD_THREADS) {
+                    const int e = 4 * (first + tid);
+                    float p[4], q[4], ahead = 0.f;
+                    load_four(x, e, a.vocab, x_step, p);
+                    load_four(y, e, a.vocab, y_step, q);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        p[i] = p_of(p[i]) - q_of(q[i]);
+                        ahead = fmaxf(ahead, p[i]);
+                    }
+                    if (ahead > 0.f && !(ahead * spare < 5.9e-8f)) {         // 1 - U is 2^-24 at least
+                        const uint4 w = philox4x32_10(make_uint4((unsigned)e >> 2, c1, stream, 2u), key2);
+                        const unsigned words[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const float u = philox_uniform(words[i]);
+                            if (p[i] > 0.f && !(1.f - u >= p[i] * spare)) b = better(b, Best{p[i] / -logf(u), e + i});
+                        }
+                    }
+                    const float best = warp_max(b.i < 0 ? 0.f : b.v);
+                    if (best > 0.f) spare = 1.001f / best;
+                }
+                b = block_best(b, best_sh);
                 cluster.sync();                              // every block runs
                 if (tid == 0) *cluster.map_shared_rank(&part_sh[rank], 0) = b;
                 cluster.sync();
                 if (rank != 0) return;
-                b = warp_best((tid & 31) < VF_CTAS ? part_sh[tid & 31] : Best{0.f, -1});
+                b = warp_best((tid & 31) < VD_CTAS ? part_sh[tid & 31] : Best{0.f, -1});
             }
             if (b.i < 0) {                                   // nothing of p lies beyond q (they differ by a rounding): p itself
-                for (int i = tid; i < a.vocab; i += VF_THREADS) race(p_of(x[i]), i);
-                b = block_best<VF_THREADS / 32>(b, best_sh);
+                for (int i = tid; i < a.vocab; i += VD_THREADS) race(p_of(x[i]), i);
+                b = block_best(b, best_sh);
             }
         }
     }
@@ -520,18 +590,22 @@ __global__ void __launch_bounds__(JUDGED ? VF_THREADS : 32) verify_kernel(VdArgs
     }
 }
 
-// How many blocks hold a row.
-int row_ctas(int vocab) {
-    int ctas = 1;
-    while (ctas < VD_MAX_CTAS && (long long)ctas * VD_SLICE < vocab) ctas *= 2;
-    return ctas;
+struct Scratch { long long parts, stats, kept, words; };      // offsets in words (32 bits)
+Scratch scratch_of(int requests, int max_drafts, int vocab, bool sampled, bool draft_logits) {
+    const long long places = draft_logits ? 2 * max_drafts + 1 : max_drafts + 1, tiles = (vocab + VD_TILE - 1) / VD_TILE;
+    Scratch s;
+    s.parts = 0;
+    s.stats = s.parts + requests * places * tiles * VD_THREADS;
+    s.kept = s.stats + (sampled ? requests * places * (long long)(sizeof(RowStats) / 4) : 0);
+    s.words = s.kept + (draft_logits ? (long long)requests * max_drafts * VD_LIST * (long long)(sizeof(Kept) / 4) : 0);
+    return s;
 }
 
 }  // namespace
 
-// Words (32 bits) of scratch a call needs, on a 16-byte boundary: what its rows leave for the kernel behind.
-TI_API long long ti_verify_scratch_words(int requests, int max_drafts, int draft_logits) {
-    return (long long)requests * ((2 * max_drafts + 1) * (long long)(sizeof(RowStats) / 4) + (draft_logits ? 2ll * VD_LIST * max_drafts : 0));
+// Words (32 bits) of scratch a call needs, on a 16-byte boundary: what its rows leave for the kernels behind.
+TI_API long long ti_verify_scratch_words(int requests, int max_drafts, int vocab, int sampled, int draft_logits) {
+    return scratch_of(requests, max_drafts, vocab, sampled != 0, draft_logits != 0).words;
 }
 
 TI_API int ti_verify_drafts(int* tokens, int* counts, float* accept, const float* logits, const int* token_ids, const int* cu_rows,
@@ -540,28 +614,22 @@ TI_API int ti_verify_drafts(int* tokens, int* counts, float* accept, const float
                             long long draft_request, long long draft_place, void* scratch, cudaStream_t stream) {
     TI_REQUIRE(rows >= 0 && vocab > 0 && requests >= 0 && requests <= 65535, "verify_drafts: bad sizes");
     TI_REQUIRE(max_drafts >= 0 && max_drafts <= VD_MAX_DRAFTS, "verify_drafts: at most %d drafts a request", VD_MAX_DRAFTS);
-    TI_REQUIRE(vocab <= VD_MAX_CTAS * VD_SLICE, "verify_drafts: at most %d tokens in the vocabulary", VD_MAX_CTAS * VD_SLICE);
+    TI_REQUIRE(vocab <= VD_MAX_VOCAB, "verify_drafts: at most %d tokens in the vocabulary", VD_MAX_VOCAB);
     TI_REQUIRE(temperature || !draft_logits, "verify_drafts: greedy requests have no use for draft logits");
     if (requests == 0) return 0;
-    RowStats* target = (RowStats*)scratch;
-    RowStats* draft = target + (size_t)requests * (max_drafts + 1);
+    const Scratch s = scratch_of(requests, max_drafts, vocab, temperature != nullptr, draft_logits != nullptr);
+    float* words = (float*)scratch;
     VdArgs a{logits, token_ids, cu_rows, temperature, topk, greedy, seed, stream_id, step, draft_logits, draft_request, draft_place,
-             target, draft, (Kept*)(draft + (size_t)requests * max_drafts), tokens, counts, accept, rows, vocab, requests, max_drafts};
-    const int ctas = row_ctas(vocab);
-    if (ctas > 8) {
-        static bool allowed[64] = {};
-        int dev = -1;
-        TI_REQUIRE(cudaGetDevice(&dev) == cudaSuccess, "verify_drafts: no device");
-        if (dev >= 64 || !allowed[dev]) {
-            TI_REQUIRE(cudaFuncSetAttribute(row_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) == cudaSuccess,
-                       "verify_drafts: clusters of %d blocks are not allowed", ctas);
-            if (dev < 64) allowed[dev] = true;
-        }
+             words + s.parts, (RowStats*)(words + s.stats), (Kept*)(words + s.kept), tokens, counts, accept, rows, vocab, requests, max_drafts,
+             (vocab + VD_TILE - 1) / VD_TILE, draft_logits ? 2 * max_drafts + 1 : max_drafts + 1};
+    ti_launch(parts_kernel, dim3(a.tiles, a.places, requests), VD_THREADS, 0, stream, a);
+    TI_CHECK_LAUNCH("verify_drafts: parts");
+    if (temperature) {
+        ti_launch(topk_kernel, dim3(a.places, requests), VD_THREADS, 0, stream, a);
+        TI_CHECK_LAUNCH("verify_drafts: top k");
     }
-    ti_launch_clusters(row_kernel, dim3(ctas, max_drafts + 1 + (draft_logits ? max_drafts : 0), requests), ctas, VD_THREADS, stream, a);
-    TI_CHECK_LAUNCH("verify_drafts: rows");
-    if (draft_logits) ti_launch_clusters(verify_kernel<true>, dim3(VF_CTAS, requests), VF_CTAS, VF_THREADS, stream, a);
-    else ti_launch(verify_kernel<false>, dim3(1, requests), 32, 0, stream, a);
+    if (draft_logits) ti_launch_clusters(verify_kernel<true>, dim3(VD_CTAS, requests), VD_CTAS, VD_THREADS, 0, stream, a);
+    else ti_launch(verify_kernel<false>, dim3(1, requests), VD_THREADS, 0, stream, a);
     TI_CHECK_LAUNCH("verify_drafts");
     return 0;
 }

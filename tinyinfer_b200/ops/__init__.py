@@ -29,7 +29,7 @@ _SIGNATURES = {
     "drafts": {
         "ti_verify_drafts": [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_void_p, c_void_p,
                              c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_ll, c_ll, c_void_p, c_void_p],
-        "ti_verify_scratch_words": [c_int, c_int, c_int],
+        "ti_verify_scratch_words": [c_int, c_int, c_int, c_int, c_int],
         "ti_ngram_drafts": [c_void_p] * 11 + [c_int] * 7 + [c_void_p],
         "ti_step_arrays": [c_void_p] * 15 + [c_int] * 9 + [c_void_p],
         "ti_step_tile_rows": [],
@@ -2458,20 +2458,20 @@ def verify_drafts(logits: torch.Tensor, token_ids: torch.Tensor, cu_rows: torch.
     out = VerifiedDrafts(torch.empty((s, d + 1), dtype=torch.int32, device=device), torch.empty((s,), dtype=torch.int32, device=device),
                          torch.empty((s, d), dtype=torch.float32, device=device))
     # scratch of the call's own: calls on several streams, or in several captured graphs, do not meet in it
-    scratch = torch.empty((_verify_scratch_words(s, d, draft_logits is not None),), dtype=torch.int32, device=device)
+    scratch = torch.empty((_verify_scratch_words(s, d, vocab, given > 0, draft_logits is not None),), dtype=torch.int32, device=device)
     _run("drafts", "ti_verify_drafts", out.tokens.data_ptr(), out.counts.data_ptr(), out.accept.data_ptr(), logits.data_ptr(),
          token_ids.data_ptr(), cu_rows.data_ptr(), n, vocab, s, d, *(_ptr(t) for t in options), _ptr(draft_logits), stride_s, stride_d,
          scratch.data_ptr(), _stream())
     return out
 
 
-def _verify_scratch_words(requests: int, max_drafts: int, draft_logits: bool) -> int:
-    key = ("verify", requests, max_drafts, draft_logits)
-    n = _scratch_floats.get(key)
+def _verify_scratch_words(*key) -> int:
+    """(requests, max_drafts, vocab, sampled, with draft logits) -> 32-bit words."""
+    n = _scratch_floats.get(("verify", *key))
     if n is None:
         fn = _fn("drafts", "ti_verify_scratch_words")
         fn.restype = ctypes.c_longlong
-        n = _scratch_floats[key] = int(fn(requests, max_drafts, draft_logits))
+        n = _scratch_floats["verify", *key] = int(fn(*key))
     return n
 
 
