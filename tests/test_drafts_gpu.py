@@ -150,6 +150,23 @@ def test_without_drafts_the_token_is_the_one_that_sample_draws(ops):
         assert got.counts.tolist() == [1] * s and bool((got.tokens[:, 1:] == -1).all()) and not got.accept.any()
 
 
+def test_where_every_draft_holds_the_next_token_is_the_one_that_sample_draws(ops):
+    """With the draft model's logits, too: no drafts, or drafts that are sure to hold (the two models' logits are the same)."""
+    for vocab, k in ((515, 0), (32003, 0), (151936, 0), (32003, 40), (20000, 1000), (9000, 5000)):
+        s, d = 12, 2
+        logits, fed = batch([d + 1] * s, vocab, seed=vocab + k, std=2.5)
+        x = logits.view(s, d + 1, vocab)
+        opts = options(s, vocab, temperature=[0.6, 1.0, 1.7] * 4, topk=[k] * s)
+        fed = ints(fed).view(s, d + 1)
+        fed[:, 1:] = x[:, :d].argmax(2).to(torch.int32)
+        for counts, rows, tokens in (([1] * s, x[:, d].contiguous(), fed[:, 0].contiguous()), ([d + 1] * s, logits, fed.flatten())):
+            got = ops.verify_drafts(rows, tokens, ints(rows_of(counts)), max_drafts=d, draft_logits=x[:, :d], **opts)
+            assert got.counts.tolist() == counts
+            want = ops.sample(x[:, d].contiguous(), *(opts[n] for n in ("temperature", "topk", "greedy", "seed", "stream_id")),
+                              opts["step"] + (counts[0] - 1))
+            assert got.tokens[:, counts[0] - 1].tolist() == want.tolist(), (vocab, k, counts[0])
+
+
 @pytest.mark.parametrize("vocab", [600, 40007])
 def test_masks_and_values_that_are_no_numbers(ops, vocab):
     """Rows that a mask leaves empty, by -inf or by the type's lowest value; infinities; NaN; drafts outside the vocabulary; drafts

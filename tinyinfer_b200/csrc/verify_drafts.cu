@@ -35,10 +35,11 @@ constexpr int VD_THREADS = 256;
 constexpr int VD_WARPS = VD_THREADS / 32;
 constexpr int VD_GROUPS = 8;         // groups of four logits a thread holds
 constexpr int VD_TILE = VD_THREADS * VD_GROUPS * 4;
-constexpr int VD_CANDIDATES = 4096;  // of a top-k row, in shared memory
+constexpr int VD_CANDIDATES = 3584;  // of a top-k row, in shared memory (14 a thread)
 constexpr int VD_MAX_VOCAB = 1 << 19;        // so many weights of at most 2^44 fit 64 bits
 constexpr int VD_LIST = 256;         // of what the threshold keeps, for the draw behind a draft that failed
 constexpr int VD_CTAS = 8;           // blocks that share such a draw
+constexpr int VD_SCAN = 4;           // groups of four tokens a thread takes at a time there
 constexpr float LOG2E = 1.4426950408889634f;
 
 // A warp's part of a row: the largest scaled logit, the sum of the exponentials relative to it, the best draw.
@@ -77,7 +78,7 @@ __device__ __forceinline__ bool is_greedy(const VdArgs& a, int r) { return a.tem
 __device__ __forceinline__ uint2 seed_of(const VdArgs& a, int r) {
     return make_uint2((unsigned)(a.seed[r] & 0xFFFFFFFFll), (unsigned)((unsigned long long)a.seed[r] >> 32));
 }
-// A place of a request: which of its rows (-1: none) and where it lies. draws: its token is wanted whatever becomes of the drafts.
+// A place of a request: which of its rows (-1: none) and where it lies. draws: its token may be wanted as the row draws it.
 struct Place { const float* x; int j; bool draws; };
 __device__ __forceinline__ Place place_of(const VdArgs& a, int r, int place, int2 rows, bool greedy) {
     const bool of_draft = place > a.max_drafts;
@@ -90,6 +91,12 @@ __device__ __forceinline__ bool has_threshold(int topk, int vocab) { return topk
 
 __device__ __forceinline__ unsigned score_key(float s) { return order_key(s + 0.f); }        // -0 and +0 are one value
 
+// 2^x, 2^-22 of itself off; nothing below 2^-126.
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
 // The weights of a row's logits, exp(v / temp - m): 2^(v * c - m * log2 e), one multiply-add and one exponential. Where that has
 // infinities on both sides (an infinite logit; a temperature whose quotients leave float32) the quotient itself is compared.
 struct Weights {
@@ -98,7 +105,7 @@ struct Weights {
     __device__ __forceinline__ Weights(float temp_, float m_) : temp(temp_), m(m_), c(LOG2E / temp_), m2(m_ * LOG2E) {
         odd = !(fabsf(m) < 1e30f) || !(c < 1e30f);
     }
-    __device__ __forceinline__ float fast(float v) const { return exp2f(fmaf(v, c, -m2)); }
+    __device__ __forceinline__ float fast(float v) const { return ex2(fmaf(v, c, -m2)); }
     __device__ __forceinline__ float quotient(float v) const {
         const float s = v / temp;
         return !(s > -INFINITY) ? 0.f : (s == m ? 1.f : expf(s - m));
@@ -108,7 +115,7 @@ struct Weights {
     __device__ __forceinline__ float spare() const { return 1.001f + fabsf(m) * 1e-6f; }
 };
 // The same of a scaled logit at hand.
-__device__ __forceinline__ float scaled_weight(float s, float m) { return !(s > -INFINITY) ? 0.f : (s == m ? 1.f : exp2f((s - m) * LOG2E)); }
+__device__ __forceinline__ float scaled_weight(float s, float m) { return !(s > -INFINITY) ? 0.f : (s == m ? 1.f : ex2((s - m) * LOG2E)); }
 
 // s + G of a scaled logit s and its uniform number.
 __device__ __forceinline__ float noisy(float s, float u) { return s - logf(-logf(u)); }
@@ -152,7 +159,9 @@ __device__ __forceinline__ void load_four(const float* x, int e, int vocab, int 
 // The tokens of thread t in a tile: groups of four, VD_THREADS groups apart.
 __device__ __forceinline__ int token_of(int tile, int t, int k) { return tile * VD_TILE + 4 * (t + k * VD_THREADS); }
 
-__global__ void __launch_bounds__(VD_THREADS, 4) parts_kernel(VdArgs a) {
+// DRAWS: open rows draw here, too (drafts that nothing judges: every row's token is wanted).
+template <bool DRAWS>
+__global__ void __launch_bounds__(VD_THREADS, DRAWS ? 4 : 5) parts_kernel(VdArgs a) {
     ti_grid_launch_dependents();
     ti_grid_wait();
     const int tid = threadIdx.x, lane = tid & 31, r = blockIdx.z;
@@ -221,7 +230,7 @@ __global__ void __launch_bounds__(VD_THREADS, 4) parts_kernel(VdArgs a) {
     }
     z = warp_sum(z);
     Best b{-INFINITY, -1};
-    if (at.draws && m > -INFINITY) {
+    if (DRAWS && m > -INFINITY) {
         // The largest of s + G, G = -log E, E = -log U. A token can pass a score B only if E < exp(s - B); E is 1 - U at least, and 1 - U
         // is exact: one comparison settles all but a few tokens once some B is known.
         const uint2 key2 = seed_of(a, r);
@@ -249,7 +258,7 @@ __global__ void __launch_bounds__(VD_THREADS, 4) parts_kernel(VdArgs a) {
                 const uint4 w = philox4x32_10(make_uint4((unsigned)i >> 2, c1, stream, 0u), key2);
                 b = better(b, Best{noisy(at.x[i] / temp, philox_uniform(word_of(w, i))), i});
             }
-            if (!weight.odd) spare = exp2f((m - warp_max(b.v)) * LOG2E) * weight.spare();
+            if (!weight.odd) spare = ex2((m - warp_max(b.v)) * LOG2E) * weight.spare();
         }
         b = warp_best(b);
     }
@@ -258,8 +267,9 @@ __global__ void __launch_bounds__(VD_THREADS, 4) parts_kernel(VdArgs a) {
 
 struct TopShared {
     alignas(16) float most[VD_THREADS];                       // read four at a time
-    unsigned key[VD_CANDIDATES];
-    int idx[VD_CANDIDATES];          // of the candidates; before them, the threads' parts that hold some
+    alignas(16) unsigned key[VD_CANDIDATES];
+    int idx[VD_CANDIDATES];
+    int part[VD_CANDIDATES];         // the threads' parts that hold candidates
     unsigned hist[256], sel[2];
     float red[33];
     Best best[VD_WARPS];
@@ -275,6 +285,7 @@ __device__ __forceinline__ float top_bound(TopShared& sh, const float* largest, 
     if (k <= VD_THREADS) {
         // every thread takes the largest of its share of them; the k-th largest of these 256, found by counting
         float own = -INFINITY;
+#pragma unroll 8
         for (int i = tid; i < n; i += VD_THREADS) own = fmaxf(own, largest[i]);
         sh.most[tid] = own;
         __syncthreads();
@@ -329,52 +340,67 @@ __global__ void __launch_bounds__(VD_THREADS) topk_kernel(VdArgs a) {
     Best b{0.f, -1};
 
     const float low = below_quotient(top_bound(sh, largest, n_largest, topk), temp);
-    for (int i = tid; i < n_largest; i += VD_THREADS) {
-        const float v = largest[i];
-        if (v >= low && v > -INFINITY) {
-            const int to = atomicAdd(&sh.parts, 1);
-            if (to < VD_CANDIDATES) sh.idx[to] = i;
-        }
+    for (int first = tid; first < n_largest; first += 8 * VD_THREADS) {         // eight loads in flight
+        float v[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v[k] = first + k * VD_THREADS < n_largest ? largest[first + k * VD_THREADS] : -INFINITY;
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+            if (v[k] >= low && v[k] > -INFINITY) {
+                const int to = atomicAdd(&sh.parts, 1);
+                if (to < VD_CANDIDATES) sh.part[to] = first + k * VD_THREADS;
+            }
     }
     __syncthreads();
-    const int n_parts = sh.parts;
-    bool fits = n_parts <= VD_CANDIDATES;
+    const int n_groups = sh.parts * VD_GROUPS;
+    bool fits = sh.parts <= VD_CANDIDATES;
     if (fits) {
-        // their logits once more, a thread a group; what reaches the bound takes the places behind them and is moved when all is found
-        for (int first = 0; first < n_parts * VD_GROUPS; first += VD_THREADS) {
-            const int w = first + tid;
-            float v[4] = {NAN, NAN, NAN, NAN};
-            int e = 0;
-            if (w < n_parts * VD_GROUPS) {
-                const int i = sh.idx[w / VD_GROUPS];
-                e = token_of(i / VD_THREADS, i % VD_THREADS, w % VD_GROUPS);
-                load_four(at.x, e, a.vocab, step, v);
+        // their logits once more, a thread a group, four in flight
+        for (int first = tid; first < n_groups; first += 4 * VD_THREADS) {
+            float v[4][4];
+            int e[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const int w = first + k * VD_THREADS;
+                e[k] = a.vocab;
+                if (w < n_groups) {
+                    const int i = sh.part[w / VD_GROUPS];
+                    e[k] = token_of(i / VD_THREADS, i % VD_THREADS, w % VD_GROUPS);
+                }
+                load_four(at.x, e[k], a.vocab, step, v[k]);
             }
 #pragma unroll
-            for (int q = 0; q < 4; ++q)
-                if (v[q] >= low && v[q] > -INFINITY) {
-                    const int to = atomicAdd(&sh.count, 1);
-                    if (to < VD_CANDIDATES) sh.key[to] = (unsigned)(e + q);
-                }
+            for (int k = 0; k < 4; ++k)
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+                    if (v[k][q] >= low && v[k][q] > -INFINITY) {
+                        const int to = atomicAdd(&sh.count, 1);
+                        if (to < VD_CANDIDATES) {
+                            sh.key[to] = score_key(v[k][q] / temp);
+                            sh.idx[to] = e[k] + q;
+                        }
+                    }
         }
         __syncthreads();
         fits = sh.count <= VD_CANDIDATES;
     }
     if (fits) {
         const int n = sh.count;
-        for (int i = tid; i < n; i += VD_THREADS) {
-            const int token = (int)sh.key[i];
-            sh.idx[i] = token;
-            sh.key[i] = score_key(at.x[token] / temp);
-        }
-        __syncthreads();
         if (n >= topk) {                                              // fewer: no finite logit of the row is missing, and all are kept
             if (n <= 2 * VD_THREADS) {
                 // the k-th largest is the key that fewer than k pass and with its equals k reach
+                if (tid < 4) sh.key[n + tid] = 0u;                    // (no key of a number is 0)
+                __syncthreads();
+                const uint4* keys = reinterpret_cast<const uint4*>(sh.key);
                 for (int i = tid; i < n; i += VD_THREADS) {
                     const unsigned own = sh.key[i];
                     int above = 0, level = 0;
-                    for (int o = 0; o < n; ++o) { above += sh.key[o] > own; level += sh.key[o] == own; }
+#pragma unroll 4
+                    for (int o = 0; o < (n + 3) / 4; ++o) {
+                        const uint4 k4 = keys[o];
+                        above += (k4.x > own) + (k4.y > own) + (k4.z > own) + (k4.w > own);
+                        level += (k4.x == own) + (k4.y == own) + (k4.z == own) + (k4.w == own);
+                    }
                     if (above < topk && topk <= above + level) sh.sel[0] = own;
                 }
                 __syncthreads();
@@ -452,12 +478,17 @@ __device__ __forceinline__ RowStats whole_row(const VdArgs& a, const Place& at, 
     const float at_draft = !greedy && drafted >= 0 && drafted < a.vocab ? at.x[drafted] : NAN;
     Best b{0.f, -1};
     float z = 0.f;
-    for (int i = lane; i < n; i += 32) {
-        const Part p = nth(i);
-        b = better(b, Best{p.v, p.i});
-        if (!greedy && p.z > 0.f) {
-            if (p.m > st.m) { z *= scaled_weight(st.m, p.m); st.m = p.m; }
-            z += p.z * scaled_weight(p.m, st.m);
+    for (int first = lane; first < n; first += 5 * 32) {     // five loads in flight
+        Part p[5];
+#pragma unroll
+        for (int k = 0; k < 5; ++k) p[k] = first + 32 * k < n ? nth(first + 32 * k) : Part{-INFINITY, 0.f, 0.f, -1};
+#pragma unroll
+        for (int k = 0; k < 5; ++k) {
+            b = better(b, Best{p[k].v, p[k].i});
+            if (!greedy && p[k].z > 0.f) {
+                if (p[k].m > st.m) { z *= scaled_weight(st.m, p[k].m); st.m = p[k].m; }
+                z += p[k].z * scaled_weight(p[k].m, st.m);
+            }
         }
     }
     st.drawn = warp_best(b).i;
@@ -522,53 +553,82 @@ __global__ void __launch_bounds__(VD_THREADS) verify_kernel(VdArgs a) {
     if (rows.y > 0) {
         const RowStats st = row_sh[held];
         b.i = st.drawn;
-        if (JUDGED && judged && held < n) {
-            const unsigned c1 = step + held;
-            const RowStats ds = row_sh[D + 1 + held];
+        const bool failed = held < n;
+        if (JUDGED && judged && (failed || !thresholded)) {
+            // What is left of p beyond q, or, if every draft held, an open row as ti_sample draws from it.
+            const unsigned c1 = step + held, domain = failed ? 2u : 0u;
+            const RowStats ds = failed ? row_sh[D + 1 + held] : RowStats{0.f, 0.f, 0u, -1, 0.f, -1, {0, 0}};
             const float* x = a.logits + (size_t)(rows.x + held) * a.vocab;
-            const float* y = a.draft_logits + r * a.draft_request + held * a.draft_place;
+            const float* y = failed ? a.draft_logits + r * a.draft_request + held * a.draft_place : x;
             const Weights pw(temp, st.m), qw(temp, ds.m);
             const float pz = st.z > 0.f ? 1.f / st.z : 0.f, qz = ds.z > 0.f ? 1.f / ds.z : 0.f;
             auto p_of = [&](float v) { return v > -INFINITY && (!st.threshold || score_key(v / temp) >= st.threshold) ? pw(v) * pz : 0.f; };
             auto q_of = [&](float v) { return v > -INFINITY && (!ds.threshold || score_key(v / temp) >= ds.threshold) ? qw(v) * qz : 0.f; };
-            // an exponential race: the largest share / E, E = -log U
+            // An exponential race, the largest share / E, E = -log U; in ti_sample's terms the largest s + G.
+            auto number = [&](int i) {
+                const uint4 w = philox4x32_10(make_uint4((unsigned)i >> 2, c1, stream, domain), key2);
+                return philox_uniform(word_of(w, i));
+            };
             auto race = [&](float share, int i) {
-                if (!(share > 0.f)) return;
-                const uint4 w = philox4x32_10(make_uint4((unsigned)i >> 2, c1, stream, 2u), key2);
-                b = better(b, Best{share / -logf(philox_uniform(word_of(w, i))), i});
+                if (share > 0.f) b = better(b, Best{share / -logf(number(i)), i});
             };
             b.i = -1;
-            if (st.listed >= 0) {                            // the threshold keeps few: the first block alone
+            if (failed && st.listed >= 0) {                  // the threshold keeps few: the first block alone
                 if (rank != 0) return;
                 const Kept* list = a.kept + ((size_t)r * D + held) * VD_LIST;
                 for (int i = tid; i < st.listed; i += VD_THREADS) race(scaled_weight(list[i].s, st.m) * pz - q_of(y[list[i].i]), list[i].i);
                 b = block_best(b, best_sh);
             } else {
-                // Only tokens whose share can still pass the best B of the warp run: share / E > B needs 1 - U < share / B.
+                // Only tokens whose share can still pass the best B of the warp run: share / E > B needs 1 - U < share / B, and 1 - U is exact.
                 cg::cluster_group cluster = cg::this_cluster();
                 const int groups = (a.vocab + 3) / 4, x_step = row_step(x), y_step = row_step(y);
+                const float room = pw.spare();
+                const bool odd = pw.odd || (failed && qw.odd);                 // every token runs
                 float spare = INFINITY;                      // 1 / B
-                for (int first = rank * VD_THREADS; first < groups; first += VD_CTAS * VD_THREADS) {
-                    const int e = 4 * (first + tid);
-                    float p[4], q[4], ahead = 0.f;
-                    load_four(x, e, a.vocab, x_step, p);
-                    load_four(y, e, a.vocab, y_step, q);
+                for (int first = rank * VD_SCAN * VD_THREADS; first < groups; first += VD_CTAS * VD_SCAN * VD_THREADS) {
+                    float p[VD_SCAN][4], q[VD_SCAN][4], ahead = 0.f;
+                    int foremost = 0;
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        p[i] = p_of(p[i]) - q_of(q[i]);
-                        ahead = fmaxf(ahead, p[i]);
+                    for (int k = 0; k < VD_SCAN; ++k) {
+                        const int e = 4 * (first + k * VD_THREADS + tid);
+                        load_four(x, e, a.vocab, x_step, p[k]);
+                        if (failed) load_four(y, e, a.vocab, y_step, q[k]);
                     }
-                    if (ahead > 0.f && !(ahead * spare < 5.9e-8f)) {         // 1 - U is 2^-24 at least
-                        const uint4 w = philox4x32_10(make_uint4((unsigned)e >> 2, c1, stream, 2u), key2);
-                        const unsigned words[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+                    for (int k = 0; k < VD_SCAN; ++k)
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
-                            const float u = philox_uniform(words[i]);
-                            if (p[i] > 0.f && !(1.f - u >= p[i] * spare)) b = better(b, Best{p[i] / -logf(u), e + i});
+                            p[k][i] = p_of(p[k][i]);
+                            if (failed) p[k][i] -= q_of(q[k][i]);
+                            if (p[k][i] > ahead) { ahead = p[k][i]; foremost = 4 * k + i; }
+                        }
+                    const int at = 4 * (first + tid);        // token 4 * k + i of the thread: at + 4 * VD_THREADS * k + i
+                    unsigned run = 0u;
+                    if (odd) {
+#pragma unroll
+                        for (int k = 0; k < VD_SCAN; ++k)
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) run |= p[k][i] > 0.f ? 1u << (4 * k + i) : 0u;
+                    } else if (spare == INFINITY) {          // nothing to beat yet: the foremost of every thread
+                        run = ahead > 0.f ? 1u << foremost : 0u;
+                    } else if (ahead * spare > 5.9e-8f) {    // 1 - U is 2^-24 at least
+#pragma unroll
+                        for (int k = 0; k < VD_SCAN; ++k) {
+                            const uint4 w = philox4x32_10(make_uint4((unsigned)(at + 4 * VD_THREADS * k) >> 2, c1, stream, domain), key2);
+                            const unsigned words[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) run |= 1.f - philox_uniform(words[i]) < p[k][i] * spare ? 1u << (4 * k + i) : 0u;
                         }
                     }
-                    const float best = warp_max(b.i < 0 ? 0.f : b.v);
-                    if (best > 0.f) spare = 1.001f / best;
+                    const bool again = spare == INFINITY && !odd;
+                    for (; run; run &= run - 1u) {           // (shares once more: the register file has no subscripts)
+                        const int bit = __ffs(run) - 1, i = at + 4 * VD_THREADS * (bit >> 2) + (bit & 3);
+                        if (failed) race(p_of(x[i]) - q_of(y[i]), i);
+                        else b = better(b, Best{noisy(x[i] / temp, number(i)), i});
+                    }
+                    const float best = warp_max(b.i < 0 ? -INFINITY : b.v);
+                    if (best > -INFINITY) spare = failed ? room / best : room * ex2((st.m - best) * LOG2E) * st.z;
+                    if (again && spare != INFINITY) first -= VD_CTAS * VD_SCAN * VD_THREADS;      // now all of these
                 }
                 b = block_best(b, best_sh);
                 cluster.sync();                              // every block runs
@@ -577,7 +637,7 @@ __global__ void __launch_bounds__(VD_THREADS) verify_kernel(VdArgs a) {
                 if (rank != 0) return;
                 b = warp_best((tid & 31) < VD_CTAS ? part_sh[tid & 31] : Best{0.f, -1});
             }
-            if (b.i < 0) {                                   // nothing of p lies beyond q (they differ by a rounding): p itself
+            if (b.i < 0 && failed) {                         // nothing of p lies beyond q (they differ by a rounding): p itself
                 for (int i = tid; i < a.vocab; i += VD_THREADS) race(p_of(x[i]), i);
                 b = block_best(b, best_sh);
             }
@@ -622,7 +682,7 @@ TI_API int ti_verify_drafts(int* tokens, int* counts, float* accept, const float
     VdArgs a{logits, token_ids, cu_rows, temperature, topk, greedy, seed, stream_id, step, draft_logits, draft_request, draft_place,
              words + s.parts, (RowStats*)(words + s.stats), (Kept*)(words + s.kept), tokens, counts, accept, rows, vocab, requests, max_drafts,
              (vocab + VD_TILE - 1) / VD_TILE, draft_logits ? 2 * max_drafts + 1 : max_drafts + 1};
-    ti_launch(parts_kernel, dim3(a.tiles, a.places, requests), VD_THREADS, 0, stream, a);
+    ti_launch(draft_logits || !temperature ? parts_kernel<false> : parts_kernel<true>, dim3(a.tiles, a.places, requests), VD_THREADS, 0, stream, a);
     TI_CHECK_LAUNCH("verify_drafts: parts");
     if (temperature) {
         ti_launch(topk_kernel, dim3(a.places, requests), VD_THREADS, 0, stream, a);
