@@ -17,8 +17,9 @@
 // Bound by reading the logits once. Three kernels:
 //   parts_kernel   streams every row, 32 logits a thread in registers, and leaves of each warp's part the largest, the sum and the best
 //                  draw, or of a top-k row each THREAD's largest logit (a 32nd of the row); no block waits for another, no warp for another.
-//   topk_kernel    a block a top-k row: the k-th largest of 256 of these largest bounds the row's k-th largest from below, so the
-//                  row's top k are in the few threads' parts (some 130 for k = 100) that reach it; those are read again and ranked.
+//   rows_kernel    a block a row. Of a top-k row: at least k of 256 of these largest logits reach a value close to the k-th largest
+//                  of the 256, which bounds the row's k-th largest from below; so the row's top k are in the few threads' parts (some
+//                  110 for k = 100) that reach it, and those are read again and ranked.
 //   verify_kernel  decides the request; behind a drawn draft that failed, clusters of blocks scan the two rows once more.
 // A row held by a cluster of 16 blocks in shared memory, threshold and sum found there, read the logits once too, but spent 13 us of a
 // block on meeting the others (a cluster's barrier 0.9 us) where its loads took 1.3: 291 us for 64 x 4 rows of 151,936 with k = 100.
@@ -60,7 +61,7 @@ struct VdArgs {
     const float* draft_logits;       // element (r, j, i) at r * draft_request + j * draft_place + i, or null
     long long draft_request, draft_place;
     float* parts;                    // [requests, places, tiles, VD_THREADS]: threads' largest logits, or warps' Parts
-    RowStats* stats;                 // [requests, places] of top-k rows
+    RowStats* stats;                 // [requests, places], where not all are greedy
     Kept* kept;                      // [requests, max_drafts, VD_LIST]
     int* tokens;                     // [requests, max_drafts + 1]
     int* counts;
@@ -265,56 +266,130 @@ __global__ void __launch_bounds__(VD_THREADS, DRAWS ? 4 : 5) parts_kernel(VdArgs
     if (lane == 0) *part = Part{m, z, b.v, b.i};
 }
 
-struct TopShared {
-    alignas(16) float most[VD_THREADS];                       // read four at a time
-    alignas(16) unsigned key[VD_CANDIDATES];
+// What a warp's parts of a row come to: all of it for the row's warp.
+__device__ __forceinline__ RowStats whole_row(const VdArgs& a, const Place& at, size_t slot, bool greedy, float temp, int drafted) {
+    const int lane = threadIdx.x & 31, n = a.tiles * VD_WARPS;
+    const Part* part = reinterpret_cast<const Part*>(a.parts + slot * a.tiles * VD_THREADS);
+    auto nth = [&](int i) { return part[(i / VD_WARPS) * (VD_THREADS / 4) + i % VD_WARPS]; };
+    RowStats st{-INFINITY, 0.f, 0u, -1, 0.f, -1, {0, 0}};
+    const float at_draft = !greedy && drafted >= 0 && drafted < a.vocab ? at.x[drafted] : NAN;
+    Best b{0.f, -1};
+    float z = 0.f;
+    for (int first = lane; first < n; first += 5 * 32) {     // five loads in flight
+        Part p[5];
+#pragma unroll
+        for (int k = 0; k < 5; ++k) p[k] = first + 32 * k < n ? nth(first + 32 * k) : Part{-INFINITY, 0.f, 0.f, -1};
+#pragma unroll
+        for (int k = 0; k < 5; ++k) {
+            b = better(b, Best{p[k].v, p[k].i});
+            if (!greedy && p[k].z > 0.f) {
+                if (p[k].m > st.m) { z *= scaled_weight(st.m, p[k].m); st.m = p[k].m; }
+                z += p[k].z * scaled_weight(p[k].m, st.m);
+            }
+        }
+    }
+    st.drawn = warp_best(b).i;
+    if (greedy) return st;
+    const float m = warp_max(st.m);
+    st.z = warp_sum(z > 0.f ? z * scaled_weight(st.m, m) : 0.f);
+    st.m = m;
+    if (at_draft > -INFINITY) st.share = Weights(temp, m)(at_draft) / st.z;
+    return st;
+}
+
+struct RowShared {
+    float most[VD_THREADS];
+    alignas(16) unsigned key[VD_CANDIDATES];                  // read four at a time
     int idx[VD_CANDIDATES];
     int part[VD_CANDIDATES];         // the threads' parts that hold candidates
     unsigned hist[256], sel[2];
     float red[33];
     Best best[VD_WARPS];
     unsigned long long total[VD_WARPS];
-    float bound;
     int parts, count, listed;
 };
 
+// The threads' largest logits of a row, number i of n at thread i % VD_THREADS: the first VD_KEPT of a thread in registers (rows of up to
+// 163,840 tokens have no more), the others read where they are wanted.
+constexpr int VD_KEPT = 20;
+struct Largest {
+    const float* of;
+    int n;
+    float kept[VD_KEPT];
+    __device__ __forceinline__ Largest(const float* of_, int n_) : of(of_), n(n_) {
+#pragma unroll
+        for (int k = 0; k < VD_KEPT; ++k) {
+            const int i = (int)threadIdx.x + k * VD_THREADS;
+            kept[k] = i < n ? of[i] : -INFINITY;
+        }
+    }
+    template <typename F> __device__ __forceinline__ void each(F f) const {
+#pragma unroll
+        for (int k = 0; k < VD_KEPT; ++k) f(kept[k]);
+        for (int i = (int)threadIdx.x + VD_KEPT * VD_THREADS; i < n; i += VD_THREADS) f(of[i]);
+    }
+};
+
 // A value that at least k of the threads' largest logits reach; -inf if there is none.
-__device__ __forceinline__ float top_bound(TopShared& sh, const float* largest, int n, int k) {
-    const int tid = threadIdx.x;
-    if (k > n) return -INFINITY;
+__device__ __forceinline__ float top_bound(RowShared& sh, const Largest& largest, int k) {
+    const int tid = threadIdx.x, lane = tid & 31;
+    if (k > largest.n) return -INFINITY;
     if (k <= VD_THREADS) {
-        // every thread takes the largest of its share of them; the k-th largest of these 256, found by counting
+        // Every thread takes the largest of its own; a value near the k-th largest of these 256 (at least k reach it, an eighth more at
+        // most unless they are equal) by halving, every warp for itself: 8 keys a lane and one addition over the warp a step. (Counting for each
+        // of the 256 how many pass it: 2,000 cycles; these steps: 500.)
         float own = -INFINITY;
-#pragma unroll 8
-        for (int i = tid; i < n; i += VD_THREADS) own = fmaxf(own, largest[i]);
+        largest.each([&](float v) { own = fmaxf(own, v); });
         sh.most[tid] = own;
         __syncthreads();
-        int above = 0, level = 0;
-        const float4* most = reinterpret_cast<const float4*>(sh.most);
-#pragma unroll 8
-        for (int i = 0; i < VD_THREADS / 4; ++i) {
-            const float4 o = most[i];
-            above += (o.x > own) + (o.y > own) + (o.z > own) + (o.w > own);
-            level += (o.x == own) + (o.y == own) + (o.z == own) + (o.w == own);
+        unsigned key[VD_WARPS], lo = ~0u, hi = 0u;
+#pragma unroll
+        for (int i = 0; i < VD_WARPS; ++i) {
+            key[i] = order_key(sh.most[lane + 32 * i]);
+            lo = min(lo, key[i]);
+            hi = max(hi, key[i]);
         }
-        if (above < k && k <= above + level) sh.bound = own;         // the same value from each that finds it
-        __syncthreads();
-        return sh.bound;
+        lo = __reduce_min_sync(~0u, lo);
+        hi = __reduce_max_sync(~0u, hi);
+        for (int reach = VD_THREADS; lo < hi && reach > k + k / 8;) {
+            const unsigned middle = lo + (hi - lo + 1) / 2;
+            int mine = 0;
+#pragma unroll
+            for (int i = 0; i < VD_WARPS; ++i) mine += key[i] >= middle;
+            mine = __reduce_add_sync(~0u, mine);
+            if (mine >= k) { lo = middle; reach = mine; }
+            else hi = middle - 1;
+        }
+        return key_value(lo);
     }
     unsigned lo = order_key(-INFINITY), hi = order_key(INFINITY);     // at least k reach lo
     for (int i = 0; i < 20 && lo < hi; ++i) {
         const unsigned middle = lo + (hi - lo + 1) / 2;
         int reach = 0;
-        for (int j = tid; j < n; j += VD_THREADS) reach += order_key(largest[j]) >= middle;
-        reach = (int)block_sum((float)reach, sh.red);                 // at most 2^24 of them: exact
+        largest.each([&](float v) { reach += order_key(v) >= middle; });
+        reach = (int)block_sum((float)reach, sh.red);                 // at most 2^14 of them: exact
         if (reach >= k) lo = middle;
         else hi = middle - 1;
     }
     return key_value(lo);
 }
 
-__global__ void __launch_bounds__(VD_THREADS) topk_kernel(VdArgs a) {
-    __shared__ TopShared sh;
+// Places in a shared list for the bits that a thread has set in `mask`: the first one's (a warp asks for all of its own at once).
+__device__ __forceinline__ int places_for(unsigned mask, int* counter) {
+    const int lane = threadIdx.x & 31, n = __popc(mask);
+    int upto = n;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int w = __shfl_up_sync(~0u, upto, o);
+        if (lane >= o) upto += w;
+    }
+    int base = 0;
+    if (lane == 31 && upto > 0) base = atomicAdd(counter, upto);
+    return __shfl_sync(~0u, base, 31) + upto - n;
+}
+
+__global__ void __launch_bounds__(VD_THREADS, 4) rows_kernel(VdArgs a) {
+    __shared__ RowShared sh;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, r = blockIdx.y, D = a.max_drafts;
     ti_grid_launch_dependents();
     if (tid == 0) sh.parts = sh.count = sh.listed = 0;
@@ -323,32 +398,44 @@ __global__ void __launch_bounds__(VD_THREADS) topk_kernel(VdArgs a) {
     const int2 rows = rows_of(a, r);
     const bool greedy = is_greedy(a, r);
     const Place at = place_of(a, r, blockIdx.x, rows, greedy);
+    if (at.j < 0) return;
+    const size_t slot = (size_t)r * a.places + blockIdx.x;
     const int topk = greedy ? 0 : a.topk[r];
-    if (at.j < 0 || !has_threshold(topk, a.vocab)) return;
-    const float temp = a.temperature[r];
+    const float temp = greedy ? 1.f : a.temperature[r];
     const int drafted = at.j < rows.y - 1 ? a.token_ids[rows.x + at.j + 1] : -1;
+    if (!has_threshold(topk, a.vocab)) {
+        if (warp > 0) return;
+        const RowStats st = whole_row(a, at, slot, greedy, temp, drafted);
+        if (lane == 0) a.stats[slot] = st;
+        return;
+    }
+    const Largest largest(a.parts + slot * a.tiles * VD_THREADS, a.tiles * VD_THREADS);
     const float at_draft = drafted >= 0 && drafted < a.vocab ? at.x[drafted] : NAN;
     const uint2 key2 = at.draws ? seed_of(a, r) : make_uint2(0u, 0u);
     const unsigned c1 = at.draws ? (unsigned)(a.step[r] + at.j) : 0u, stream = at.draws ? (unsigned)a.stream_id[r] : 0u;
-    const size_t slot = (size_t)r * a.places + blockIdx.x;
-    const float* largest = a.parts + slot * a.tiles * VD_THREADS;
-    const int n_largest = a.tiles * VD_THREADS, step = row_step(at.x);
+    const int step = row_step(at.x);
     const bool lists = !at.draws && (int)blockIdx.x <= D;             // a draw behind a failed draft may want them
     Kept* kept = lists ? a.kept + ((size_t)r * D + at.j) * VD_LIST : nullptr;
     RowStats st{0.f, 0.f, 0u, -1, 0.f, -1, {0, 0}};
     unsigned long long sum = 0;                                       // weights of at most 1 in steps of 2^-44
     Best b{0.f, -1};
 
-    const float low = below_quotient(top_bound(sh, largest, n_largest, topk), temp);
-    for (int first = tid; first < n_largest; first += 8 * VD_THREADS) {         // eight loads in flight
-        float v[8];
+    const float low = below_quotient(top_bound(sh, largest, topk), temp);
+    {
+        unsigned hits = 0u;
 #pragma unroll
-        for (int k = 0; k < 8; ++k) v[k] = first + k * VD_THREADS < n_largest ? largest[first + k * VD_THREADS] : -INFINITY;
+        for (int k = 0; k < VD_KEPT; ++k) hits |= largest.kept[k] >= low && largest.kept[k] > -INFINITY ? 1u << k : 0u;
+        int to = places_for(hits, &sh.parts);
 #pragma unroll
-        for (int k = 0; k < 8; ++k)
-            if (v[k] >= low && v[k] > -INFINITY) {
-                const int to = atomicAdd(&sh.parts, 1);
-                if (to < VD_CANDIDATES) sh.part[to] = first + k * VD_THREADS;
+        for (int k = 0; k < VD_KEPT; ++k)
+            if (hits >> k & 1u) {
+                if (to < VD_CANDIDATES) sh.part[to] = tid + k * VD_THREADS;
+                ++to;
+            }
+        for (int i = tid + VD_KEPT * VD_THREADS; i < largest.n; i += VD_THREADS)
+            if (largest.of[i] >= low && largest.of[i] > -INFINITY) {
+                to = atomicAdd(&sh.parts, 1);
+                if (to < VD_CANDIDATES) sh.part[to] = i;
             }
     }
     __syncthreads();
@@ -356,12 +443,12 @@ __global__ void __launch_bounds__(VD_THREADS) topk_kernel(VdArgs a) {
     bool fits = sh.parts <= VD_CANDIDATES;
     if (fits) {
         // their logits once more, a thread a group, four in flight
-        for (int first = tid; first < n_groups; first += 4 * VD_THREADS) {
+        for (int first = 0; first < n_groups; first += 4 * VD_THREADS) {
             float v[4][4];
             int e[4];
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-                const int w = first + k * VD_THREADS;
+                const int w = first + k * VD_THREADS + tid;
                 e[k] = a.vocab;
                 if (w < n_groups) {
                     const int i = sh.part[w / VD_GROUPS];
@@ -369,16 +456,22 @@ __global__ void __launch_bounds__(VD_THREADS) topk_kernel(VdArgs a) {
                 }
                 load_four(at.x, e[k], a.vocab, step, v[k]);
             }
+            unsigned hits = 0u;
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+#pragma unroll
+                for (int q = 0; q < 4; ++q) hits |= v[k][q] >= low && v[k][q] > -INFINITY ? 1u << (4 * k + q) : 0u;
+            int to = places_for(hits, &sh.count);
 #pragma unroll
             for (int k = 0; k < 4; ++k)
 #pragma unroll
                 for (int q = 0; q < 4; ++q)
-                    if (v[k][q] >= low && v[k][q] > -INFINITY) {
-                        const int to = atomicAdd(&sh.count, 1);
+                    if (hits >> (4 * k + q) & 1u) {
                         if (to < VD_CANDIDATES) {
-                            sh.key[to] = score_key(v[k][q] / temp);
+                            sh.key[to] = __float_as_uint(v[k][q]);
                             sh.idx[to] = e[k] + q;
                         }
+                        ++to;
                     }
         }
         __syncthreads();
@@ -386,38 +479,38 @@ __global__ void __launch_bounds__(VD_THREADS) topk_kernel(VdArgs a) {
     }
     if (fits) {
         const int n = sh.count;
-        if (n >= topk) {                                              // fewer: no finite logit of the row is missing, and all are kept
-            if (n <= 2 * VD_THREADS) {
-                // the k-th largest is the key that fewer than k pass and with its equals k reach
-                if (tid < 4) sh.key[n + tid] = 0u;                    // (no key of a number is 0)
-                __syncthreads();
-                const uint4* keys = reinterpret_cast<const uint4*>(sh.key);
-                for (int i = tid; i < n; i += VD_THREADS) {
-                    const unsigned own = sh.key[i];
-                    int above = 0, level = 0;
+        for (int i = tid; i < n; i += VD_THREADS) sh.key[i] = score_key(__uint_as_float(sh.key[i]) / temp);
+        if (tid < 4 && n + tid < VD_CANDIDATES) sh.key[n + tid] = 0u;         // (no key of a number is 0)
+        if (tid == 0) sh.sel[0] = sh.sel[1] = 0u;
+        __syncthreads();
+        if (n <= 2 * VD_THREADS) {
+            // the k-th largest is the key that fewer than k pass and with its equals k reach; fewer than k in all: no finite logit of
+            // the row is missing, and all are kept
+            const uint4* keys = reinterpret_cast<const uint4*>(sh.key);
+            for (int i = tid; i < n; i += VD_THREADS) {
+                const unsigned own = sh.key[i];
+                int above = 0, level = 0;
 #pragma unroll 4
-                    for (int o = 0; o < (n + 3) / 4; ++o) {
-                        const uint4 k4 = keys[o];
-                        above += (k4.x > own) + (k4.y > own) + (k4.z > own) + (k4.w > own);
-                        level += (k4.x == own) + (k4.y == own) + (k4.z == own) + (k4.w == own);
-                    }
-                    if (above < topk && topk <= above + level) sh.sel[0] = own;
+                for (int o = 0; o < (n + 3) / 4; ++o) {
+                    const uint4 k4 = keys[o];
+                    above += (k4.x > own) + (k4.y > own) + (k4.z > own) + (k4.w > own);
+                    level += (k4.x == own) + (k4.y == own) + (k4.z == own) + (k4.w == own);
                 }
-                __syncthreads();
-                st.threshold = sh.sel[0];
-            } else {
+                if (above < topk && topk <= above + level) sh.sel[0] = own;
+                if (above == 0) sh.sel[1] = own;
+            }
+            __syncthreads();
+            st.threshold = sh.sel[0];
+            st.m = n > 0 ? key_value(sh.sel[1]) : -INFINITY;
+        } else {
+            if (n >= topk)
                 st.threshold = select_kth(topk, sh.hist, sh.sel, [&](auto count) {
                     for (int i = tid; i < n; i += VD_THREADS) count(sh.key[i]);
                 });
-            }
+            float top = -INFINITY;
+            for (int i = tid; i < n; i += VD_THREADS) top = fmaxf(top, key_value(sh.key[i]));
+            st.m = block_max(top, sh.red);
         }
-        unsigned top = 0u;
-        for (int i = tid; i < n; i += VD_THREADS) top = max(top, sh.key[i]);
-        top = __reduce_max_sync(~0u, top);
-        if (lane == 0) sh.most[warp] = __uint_as_float(top);
-        __syncthreads();
-        top = __reduce_max_sync(~0u, lane < VD_WARPS ? __float_as_uint(sh.most[lane]) : 0u);
-        st.m = n > 0 ? key_value(top) : -INFINITY;
         for (int i = tid; i < n; i += VD_THREADS) {
             if (sh.key[i] < st.threshold) continue;
             const float s = key_value(sh.key[i]);
@@ -455,11 +548,15 @@ __global__ void __launch_bounds__(VD_THREADS) topk_kernel(VdArgs a) {
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
-    if (lane == 0) sh.total[warp] = sum;
-    b = block_best(b, sh.best);
-    if (tid == 0) {
-        sum = 0;
-        for (int w = 0; w < VD_WARPS; ++w) sum += sh.total[w];
+    b = warp_best(b);
+    if (lane == 0) { sh.total[warp] = sum; sh.best[warp] = b; }
+    __syncthreads();
+    if (warp > 0) return;
+    sum = lane < VD_WARPS ? sh.total[lane] : 0;
+#pragma unroll
+    for (int o = VD_WARPS / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
+    b = warp_best(lane < VD_WARPS ? sh.best[lane] : Best{0.f, -1});
+    if (lane == 0) {
         st.z = (float)((double)sum * (1.0 / 17592186044416.0));
         st.drawn = b.i;
         const float s = at_draft / temp;
@@ -469,41 +566,10 @@ __global__ void __launch_bounds__(VD_THREADS) topk_kernel(VdArgs a) {
     }
 }
 
-// What a warp's parts of a row come to: all of it for the row's warp.
-__device__ __forceinline__ RowStats whole_row(const VdArgs& a, const Place& at, size_t slot, bool greedy, float temp, int drafted) {
-    const int lane = threadIdx.x & 31, n = a.tiles * VD_WARPS;
-    const Part* part = reinterpret_cast<const Part*>(a.parts + slot * a.tiles * VD_THREADS);
-    auto nth = [&](int i) { return part[(i / VD_WARPS) * (VD_THREADS / 4) + i % VD_WARPS]; };
-    RowStats st{-INFINITY, 0.f, 0u, -1, 0.f, -1, {0, 0}};
-    const float at_draft = !greedy && drafted >= 0 && drafted < a.vocab ? at.x[drafted] : NAN;
-    Best b{0.f, -1};
-    float z = 0.f;
-    for (int first = lane; first < n; first += 5 * 32) {     // five loads in flight
-        Part p[5];
-#pragma unroll
-        for (int k = 0; k < 5; ++k) p[k] = first + 32 * k < n ? nth(first + 32 * k) : Part{-INFINITY, 0.f, 0.f, -1};
-#pragma unroll
-        for (int k = 0; k < 5; ++k) {
-            b = better(b, Best{p[k].v, p[k].i});
-            if (!greedy && p[k].z > 0.f) {
-                if (p[k].m > st.m) { z *= scaled_weight(st.m, p[k].m); st.m = p[k].m; }
-                z += p[k].z * scaled_weight(p[k].m, st.m);
-            }
-        }
-    }
-    st.drawn = warp_best(b).i;
-    if (greedy) return st;
-    const float m = warp_max(st.m);
-    st.z = warp_sum(z > 0.f ? z * scaled_weight(st.m, m) : 0.f);
-    st.m = m;
-    if (at_draft > -INFINITY) st.share = Weights(temp, m)(at_draft) / st.z;
-    return st;
-}
-
 // Decides the request by its rows; if a drawn draft failed, draws from what is left of p beyond q. JUDGED: a cluster of blocks a
-// request, which share that draw's rows out; otherwise a block.
-template <bool JUDGED>
-__global__ void __launch_bounds__(VD_THREADS) verify_kernel(VdArgs a) {
+// request, which share that draw's rows out; otherwise a block. GREEDY: every request is, and the rows' parts are met here.
+template <bool JUDGED, bool GREEDY>
+__global__ void __launch_bounds__(VD_THREADS, 4) verify_kernel(VdArgs a) {
     __shared__ RowStats row_sh[2 * VD_MAX_DRAFTS + 1];
     __shared__ Best best_sh[VD_WARPS], part_sh[VD_CTAS];
     __shared__ int held_sh;
@@ -512,7 +578,7 @@ __global__ void __launch_bounds__(VD_THREADS) verify_kernel(VdArgs a) {
     const int r = blockIdx.y, tid = threadIdx.x, D = a.max_drafts, rank = blockIdx.x;
     const int2 rows = rows_of(a, r);
     int* out = a.tokens + (size_t)r * (D + 1);
-    const bool greedy = is_greedy(a, r);
+    const bool greedy = GREEDY || is_greedy(a, r);
     const int n = rows.y - 1;
     const bool judged = JUDGED && !greedy;                   // by the ratio of the probabilities
     const float temp = greedy ? 1.f : a.temperature[r];
@@ -520,13 +586,13 @@ __global__ void __launch_bounds__(VD_THREADS) verify_kernel(VdArgs a) {
     const uint2 key2 = judged ? seed_of(a, r) : make_uint2(0u, 0u);
     const unsigned step = judged ? (unsigned)a.step[r] : 0u, stream = judged ? (unsigned)a.stream_id[r] : 0u;
     const int fed = tid < n ? a.token_ids[rows.x + tid + 1] : -1;     // the draft of lane tid
-    for (int place = tid >> 5; place < a.places; place += VD_WARPS) {
-        const Place at = place_of(a, r, place, rows, greedy);
-        if (at.j < 0) continue;
-        const size_t slot = (size_t)r * a.places + place;
-        const RowStats st = thresholded ? a.stats[slot]
-                                        : whole_row(a, at, slot, greedy, temp, at.j < n ? a.token_ids[rows.x + at.j + 1] : -1);
-        if ((tid & 31) == 0) row_sh[place] = st;
+    if (GREEDY) {
+        for (int place = tid >> 5; place < rows.y; place += VD_WARPS) {
+            const RowStats st = whole_row(a, place_of(a, r, place, rows, true), (size_t)r * a.places + place, true, 1.f, -1);
+            if ((tid & 31) == 0) row_sh[place] = st;
+        }
+    } else if (tid < a.places && place_of(a, r, tid, rows, greedy).j >= 0) {
+        row_sh[tid] = a.stats[(size_t)r * a.places + tid];
     }
     __syncthreads();
     if (tid < 32) {
@@ -579,56 +645,68 @@ __global__ void __launch_bounds__(VD_THREADS) verify_kernel(VdArgs a) {
                 for (int i = tid; i < st.listed; i += VD_THREADS) race(scaled_weight(list[i].s, st.m) * pz - q_of(y[list[i].i]), list[i].i);
                 b = block_best(b, best_sh);
             } else {
-                // Only tokens whose share can still pass the best B of the warp run: share / E > B needs 1 - U < share / B, and 1 - U is exact.
                 cg::cluster_group cluster = cg::this_cluster();
                 const int groups = (a.vocab + 3) / 4, x_step = row_step(x), y_step = row_step(y);
-                const float room = pw.spare();
-                const bool odd = pw.odd || (failed && qw.odd);                 // every token runs
+                // Logits of both rows that no threshold and no infinity cuts: a multiply-add and an exponential each. Otherwise, every
+                // token by p_of and q_of.
+                const bool plain = !st.threshold && !ds.threshold && !pw.odd && !(failed && qw.odd) && st.z > 0.f;
+                // Only tokens whose share can still pass the best B of the warp run: share / E > B needs 1 - U < share / B, and 1 - U is exact.
                 float spare = INFINITY;                      // 1 / B
                 for (int first = rank * VD_SCAN * VD_THREADS; first < groups; first += VD_CTAS * VD_SCAN * VD_THREADS) {
+                    const int at = 4 * (first + tid);        // token 4 * k + i of the thread: at + 4 * VD_THREADS * k + i
                     float p[VD_SCAN][4], q[VD_SCAN][4], ahead = 0.f;
-                    int foremost = 0;
 #pragma unroll
-                    for (int k = 0; k < VD_SCAN; ++k) {
-                        const int e = 4 * (first + k * VD_THREADS + tid);
-                        load_four(x, e, a.vocab, x_step, p[k]);
-                        if (failed) load_four(y, e, a.vocab, y_step, q[k]);
+                    for (int k = 0; k < VD_SCAN; ++k) load_four(x, at + 4 * VD_THREADS * k, a.vocab, x_step, p[k]);
+                    if (failed) {
+#pragma unroll
+                        for (int k = 0; k < VD_SCAN; ++k) load_four(y, at + 4 * VD_THREADS * k, a.vocab, y_step, q[k]);
                     }
 #pragma unroll
                     for (int k = 0; k < VD_SCAN; ++k)
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
-                            p[k][i] = p_of(p[k][i]);
-                            if (failed) p[k][i] -= q_of(q[k][i]);
-                            if (p[k][i] > ahead) { ahead = p[k][i]; foremost = 4 * k + i; }
+                            if (plain) {
+                                p[k][i] = pw.fast(fmaxf(p[k][i], -INFINITY)) * pz;
+                                if (failed) p[k][i] = fmaf(-qz, qw.fast(fmaxf(q[k][i], -INFINITY)), p[k][i]);
+                            } else {
+                                p[k][i] = p_of(p[k][i]);
+                                if (failed) p[k][i] -= q_of(q[k][i]);
+                            }
+                            ahead = fmaxf(ahead, p[k][i]);
                         }
-                    const int at = 4 * (first + tid);        // token 4 * k + i of the thread: at + 4 * VD_THREADS * k + i
-                    unsigned run = 0u;
-                    if (odd) {
+                    bool again = false;
+                    do {
+                        unsigned run = 0u;
+                        again = plain && spare == INFINITY;  // nothing to beat yet: the foremost of every thread, then all
+                        if (again || !plain) {
 #pragma unroll
-                        for (int k = 0; k < VD_SCAN; ++k)
+                            for (int k = 0; k < VD_SCAN; ++k)
 #pragma unroll
-                            for (int i = 0; i < 4; ++i) run |= p[k][i] > 0.f ? 1u << (4 * k + i) : 0u;
-                    } else if (spare == INFINITY) {          // nothing to beat yet: the foremost of every thread
-                        run = ahead > 0.f ? 1u << foremost : 0u;
-                    } else if (ahead * spare > 5.9e-8f) {    // 1 - U is 2^-24 at least
+                                for (int i = 0; i < 4; ++i) run |= p[k][i] > 0.f && (p[k][i] == ahead || !plain) ? 1u << (4 * k + i) : 0u;
+                        } else if (ahead * spare > 5.9e-8f) {                // 1 - U is 2^-24 at least
 #pragma unroll
-                        for (int k = 0; k < VD_SCAN; ++k) {
-                            const uint4 w = philox4x32_10(make_uint4((unsigned)(at + 4 * VD_THREADS * k) >> 2, c1, stream, domain), key2);
-                            const unsigned words[4] = {w.x, w.y, w.z, w.w};
+                            for (int k = 0; k < VD_SCAN; ++k) {
+                                const uint4 w = philox4x32_10(make_uint4((unsigned)(at + 4 * VD_THREADS * k) >> 2, c1, stream, domain), key2);
+                                const unsigned words[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-                            for (int i = 0; i < 4; ++i) run |= 1.f - philox_uniform(words[i]) < p[k][i] * spare ? 1u << (4 * k + i) : 0u;
+                                for (int i = 0; i < 4; ++i) run |= 1.f - philox_uniform(words[i]) < p[k][i] * spare ? 1u << (4 * k + i) : 0u;
+                            }
                         }
-                    }
-                    const bool again = spare == INFINITY && !odd;
-                    for (; run; run &= run - 1u) {           // (shares once more: the register file has no subscripts)
-                        const int bit = __ffs(run) - 1, i = at + 4 * VD_THREADS * (bit >> 2) + (bit & 3);
-                        if (failed) race(p_of(x[i]) - q_of(y[i]), i);
-                        else b = better(b, Best{noisy(x[i] / temp, number(i)), i});
-                    }
-                    const float best = warp_max(b.i < 0 ? -INFINITY : b.v);
-                    if (best > -INFINITY) spare = failed ? room / best : room * ex2((st.m - best) * LOG2E) * st.z;
-                    if (again && spare != INFINITY) first -= VD_CTAS * VD_SCAN * VD_THREADS;      // now all of these
+                        for (; run; run &= run - 1u) {
+                            const int bit = __ffs(run) - 1, i = at + 4 * VD_THREADS * (bit >> 2) + (bit & 3);
+                            if (failed) {
+                                float share = 0.f;           // the register file has no subscripts
+#pragma unroll
+                                for (int o = 0; o < 4 * VD_SCAN; ++o) share = bit == o ? p[o >> 2][o & 3] : share;
+                                race(share, i);
+                            } else {
+                                b = better(b, Best{noisy(x[i] / temp, number(i)), i});
+                            }
+                        }
+                        const float best = warp_max(b.i < 0 ? -INFINITY : b.v);
+                        if (best > -INFINITY) spare = pw.spare() * (failed ? 1.f / best : ex2((st.m - best) * LOG2E) * st.z);
+                        again = again && spare != INFINITY;
+                    } while (again);
                 }
                 b = block_best(b, best_sh);
                 cluster.sync();                              // every block runs
@@ -685,11 +763,11 @@ TI_API int ti_verify_drafts(int* tokens, int* counts, float* accept, const float
     ti_launch(draft_logits || !temperature ? parts_kernel<false> : parts_kernel<true>, dim3(a.tiles, a.places, requests), VD_THREADS, 0, stream, a);
     TI_CHECK_LAUNCH("verify_drafts: parts");
     if (temperature) {
-        ti_launch(topk_kernel, dim3(a.places, requests), VD_THREADS, 0, stream, a);
-        TI_CHECK_LAUNCH("verify_drafts: top k");
+        ti_launch(rows_kernel, dim3(a.places, requests), VD_THREADS, 0, stream, a);
+        TI_CHECK_LAUNCH("verify_drafts: rows");
     }
-    if (draft_logits) ti_launch_clusters(verify_kernel<true>, dim3(VD_CTAS, requests), VD_CTAS, VD_THREADS, 0, stream, a);
-    else ti_launch(verify_kernel<false>, dim3(1, requests), VD_THREADS, 0, stream, a);
+    if (draft_logits) ti_launch_clusters(verify_kernel<true, false>, dim3(VD_CTAS, requests), VD_CTAS, VD_THREADS, 0, stream, a);
+    else ti_launch(temperature ? verify_kernel<false, false> : verify_kernel<false, true>, dim3(1, requests), VD_THREADS, 0, stream, a);
     TI_CHECK_LAUNCH("verify_drafts");
     return 0;
 }
