@@ -2,16 +2,26 @@
 // that ends in front of place e (1 <= e < n) is l(e) = the largest l <= max_match with h[e-l .. e) = h[n-l .. n). The place with the
 // longest match of at least min_match tokens is taken, of several the latest, and the text is drafted to go on as it did there:
 // draft t = h[e + t mod (n - e)] (a repetition shorter than the drafts repeats). One comparison decides most places, so the kernel
-// reads the text once and is bound by that.
-#include "common.cuh"
+// reads the text once, 16 bytes a lane and eight loads in flight, and is bound by that; a long text is shared out over a cluster of
+// blocks, whose best places (longest, then latest: the larger of two 64-bit numbers, in any order) meet in the first one's shared memory.
+#include <cooperative_groups.h>
+
+#include "draws.cuh"
+
+namespace cg = cooperative_groups;
 
 namespace {
 
-constexpr int NG_THREADS = 512;
+constexpr int NG_THREADS = 256;
+constexpr int NG_WARPS = NG_THREADS / 32;
 constexpr int NG_MAX_MATCH = 32;
+constexpr int NG_MAX_NEW = 512;
+constexpr int NG_CTAS = 8;
+constexpr int NG_LEAST = 4096;       // a row of so many tokens, times the blocks it has, gets twice the blocks
+constexpr int NG_LOADS = 8;
 
 struct NgArgs {
-    int* history;                    // [rows, room], row stride `room`
+    int* history;                    // [rows, room]
     const int* lengths;              // per request
     const int* state_slots;          // row of the history of each request, or null: its number
     const int* new_tokens;           // [requests, new_width] or null
@@ -33,51 +43,84 @@ __device__ __forceinline__ unsigned long long warp_max64(unsigned long long v) {
 }
 
 __global__ void __launch_bounds__(NG_THREADS) ngram_kernel(NgArgs a) {
-    __shared__ unsigned long long best_sh[NG_THREADS / 32];
+    __shared__ unsigned long long best_sh[NG_WARPS], part_sh[NG_CTAS];
     __shared__ int last_sh[NG_MAX_MATCH];
     ti_grid_launch_dependents();
     ti_grid_wait();
-    const int r = blockIdx.x, tid = threadIdx.x, D = a.max_drafts;
-    int* out = a.tokens + (size_t)r * (D + 1);
+    const int r = blockIdx.y, rank = blockIdx.x, ctas = gridDim.x, tid = threadIdx.x, D = a.max_drafts;
     const int row = a.state_slots ? a.state_slots[r] : r;
     const int held = a.lengths[r];
     const int brought = a.new_tokens ? min(max(a.new_counts[r], 0), a.new_width) : 0;
     const bool known = row >= 0 && row < a.rows && held >= 0 && held <= a.room;
     const bool fits = known && brought <= a.room - held;
-    if (tid == 0 && !fits && a.status) atomicExch(a.status, 6);       // a text without a row, or longer than its row
     int* h = a.history + (size_t)(known ? row : 0) * a.room;
+    const int* fresh = a.new_tokens + (size_t)r * a.new_width;
     const int n = fits ? held + brought : (known ? held : 0);
-    if (fits && tid < brought) h[held + tid] = a.new_tokens[(size_t)r * a.new_width + tid];
+    const bool there = fits && n > 0;
+    auto token = [&](int i) { return i < held ? h[i] : fresh[i - held]; };        // nobody waits for the new ones to be written
+    if (there && tid < a.max_match && tid < n) last_sh[tid] = token(n - 1 - tid);
     __syncthreads();
     unsigned long long best = 0;
-    if (fits && n > 0) {
-        if (tid < a.max_match) last_sh[tid] = n - 1 - tid >= 0 ? h[n - 1 - tid] : 0;
-        __syncthreads();
-        for (int e = 1 + tid; e < n; e += NG_THREADS) {
-            int l = 0;
-            while (l < a.max_match && l < e && h[e - 1 - l] == last_sh[l]) ++l;
-            if (l >= a.min_match) {
-                const unsigned long long key = ((unsigned long long)l << 32) | (unsigned)e;
-                best = key > best ? key : best;
+    if (there && n > 1) {
+        const int last = last_sh[0];
+        auto look = [&](int i, int value) {                  // the match that ends with token i
+            if (value != last) return;
+            int l = 1;
+            while (l < a.max_match && l <= i && token(i - l) == last_sh[l]) ++l;
+            const unsigned long long key = ((unsigned long long)l << 32) | (unsigned)(i + 1);
+            if (l >= a.min_match && key > best) best = key;
+        };
+        // tokens 0 .. end - 1 as they lie; group g has those from 4 g - shift on
+        const int end = min(held, n - 1), shift = (int)(((uintptr_t)h >> 2) & 3), groups = (end + shift + 3) >> 2;
+        const int4* from = reinterpret_cast<const int4*>(h - shift);
+        for (int first = rank * NG_LOADS * NG_THREADS + tid; first < groups; first += ctas * NG_LOADS * NG_THREADS) {
+            int4 v[NG_LOADS];
+#pragma unroll
+            for (int k = 0; k < NG_LOADS; ++k) {
+                const int g = first + k * NG_THREADS, i = 4 * g - shift;
+                if (i >= 0 && i + 3 < end) {
+                    v[k] = from[g];
+                } else {                                     // the text's ends, and behind them (a token that is not `last`)
+                    v[k].x = i >= 0 && i < end ? h[i] : ~last;
+                    v[k].y = i + 1 >= 0 && i + 1 < end ? h[i + 1] : ~last;
+                    v[k].z = i + 2 >= 0 && i + 2 < end ? h[i + 2] : ~last;
+                    v[k].w = i + 3 >= 0 && i + 3 < end ? h[i + 3] : ~last;
+                }
+            }
+#pragma unroll
+            for (int k = 0; k < NG_LOADS; ++k) {
+                const int i = 4 * (first + k * NG_THREADS) - shift;
+                if (v[k].x != last && v[k].y != last && v[k].z != last && v[k].w != last) continue;
+                look(i, v[k].x); look(i + 1, v[k].y); look(i + 2, v[k].z); look(i + 3, v[k].w);
             }
         }
+        if (rank == 0)                                       // the new ones but the last
+            for (int i = held + tid; i < n - 1; i += NG_THREADS) look(i, token(i));
     }
     best = warp_max64(best);
     if ((tid & 31) == 0) best_sh[tid >> 5] = best;
     __syncthreads();
-    if (tid < 32) {
-        best = warp_max64(tid < NG_THREADS / 32 ? best_sh[tid] : 0ull);
-        const int e = (int)(best & 0xFFFFFFFFull);
-        const bool there = fits && n > 0;
-        const int most = a.limits ? min(max(a.limits[r], 0), D) : D;
-        const int drafts = there && best ? most : 0;
-        for (int t = tid; t <= D; t += 32) out[t] = t == 0 ? (there ? h[n - 1] : -1) : (t <= drafts ? h[e + (t - 1) % (n - e)] : -1);
-        if (tid == 0) {
-            a.counts[r] = there ? 1 + drafts : 0;
-            a.starts[r] = there ? n - 1 : 0;
-            a.lengths_out[r] = n;
-        }
+    best = warp_max64((tid & 31) < NG_WARPS ? best_sh[tid & 31] : 0ull);
+    if (ctas > 1) {
+        cg::cluster_group cluster = cg::this_cluster();
+        cluster.sync();                                      // every block runs
+        if (tid == 0) *cluster.map_shared_rank(&part_sh[rank], 0) = best;
+        cluster.sync();
+        if (rank != 0) return;
+        best = warp_max64((tid & 31) < ctas ? part_sh[tid & 31] : 0ull);
     }
+    const int e = (int)(best & 0xFFFFFFFFull);
+    const int most = a.limits ? min(max(a.limits[r], 0), D) : D;
+    const int drafts = there && best ? most : 0;
+    if (tid <= D) a.tokens[(size_t)r * (D + 1) + tid] = tid == 0 ? (there ? last_sh[0] : -1) : (tid <= drafts ? token(e + (tid - 1) % (n - e)) : -1);
+    if (tid == 0) {
+        a.counts[r] = there ? 1 + drafts : 0;
+        a.starts[r] = there ? n - 1 : 0;
+        a.lengths_out[r] = n;
+        if (!fits && a.status) atomicExch(a.status, 6);      // a text without a row, or longer than its row
+    }
+    if (fits)
+        for (int i = tid; i < brought; i += NG_THREADS) h[held + i] = fresh[i];
 }
 
 }  // namespace
@@ -85,13 +128,15 @@ __global__ void __launch_bounds__(NG_THREADS) ngram_kernel(NgArgs a) {
 TI_API int ti_ngram_drafts(int* tokens, int* counts, int* starts, int* lengths_out, int* history, const int* lengths, const int* state_slots,
                            const int* new_tokens, const int* new_counts, const int* limits, int* status, int requests, int rows, int room,
                            int new_width, int max_drafts, int min_match, int max_match, cudaStream_t stream) {
-    TI_REQUIRE(requests >= 0 && requests <= 65535 && rows >= 0 && room >= 0 && max_drafts >= 0 && new_width >= 0 && new_width <= NG_THREADS,
-               "ngram_drafts: bad sizes");
+    TI_REQUIRE(requests >= 0 && requests <= 65535 && rows >= 0 && room >= 0 && new_width >= 0 && new_width <= NG_MAX_NEW, "ngram_drafts: bad sizes");
+    TI_REQUIRE(max_drafts >= 0 && max_drafts < NG_THREADS, "ngram_drafts: at most %d drafts", NG_THREADS - 1);
     TI_REQUIRE(min_match >= 1 && max_match >= min_match && max_match <= NG_MAX_MATCH, "ngram_drafts: matches of 1 to %d tokens", NG_MAX_MATCH);
     if (requests == 0) return 0;
     NgArgs a{history, lengths, state_slots, new_tokens, new_counts, limits, tokens, counts, starts, lengths_out, status,
              requests, rows, room, new_width, max_drafts, min_match, max_match};
-    ti_launch(ngram_kernel, requests, NG_THREADS, 0, stream, a);
+    int ctas = 1;
+    while (ctas < NG_CTAS && ctas * NG_LEAST < room) ctas *= 2;
+    ti_launch_clusters(ngram_kernel, dim3(ctas, requests), ctas, NG_THREADS, 0, stream, a);
     TI_CHECK_LAUNCH("ngram_drafts");
     return 0;
 }

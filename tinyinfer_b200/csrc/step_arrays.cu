@@ -114,7 +114,9 @@ TI_API int ti_step_arrays(int* token_ids, int* positions, int* token_seq, int* c
     SaArgs a{starts, counts, state_slots, tables, tokens, token_ids, positions, token_seq, cache_slots, cu_seqlens, q_starts, context_lens,
              (int4*)tiles, block_tables, status, requests, groups, table_rows, width, token_width, rows, max_count,
              (max_count + SA_TILE - 1) / SA_TILE, page_size, pad_page};
-    ti_launch(step_arrays_kernel, dim3(1, requests + 1), SA_THREADS, 0, stream, a);
+    // blocks a request: as many as keep a thread at four tokens and sixteen words of each table
+    const int parts = max(1, min(64, max((max_count + 4 * SA_THREADS - 1) / (4 * SA_THREADS), (width + 16 * SA_THREADS - 1) / (16 * SA_THREADS))));
+    ti_launch(step_arrays_kernel, dim3(parts, requests + 1), SA_THREADS, 0, stream, a);
     TI_CHECK_LAUNCH("step_arrays");
     return 0;
 }

@@ -2391,13 +2391,37 @@ def _on_current(device) -> None:
 
 
 def _per_request(n: int, device, **tensors) -> None:
-    """Checks tensors of one entry a request on one device."""
+    """Checks tensors of one entry a request on one device: ``name=(tensor, dtype)``."""
     for name, (t, dtype) in tensors.items():
+        if isinstance(t, torch.Tensor) and t.dtype is dtype and t.shape == (n,) and t.device == device and t.is_contiguous():
+            continue
         _check(t, name, dtype, 1)
         if t.shape[0] != n:
             raise KernelError(f"{name} must have one entry per request: {n}, got {t.shape[0]}")
-        if t.device != device:
-            raise KernelError(f"{name} lies on {t.device}, the others on {device}")
+        raise KernelError(f"{name} lies on {t.device}, the others on {device}")
+
+
+_layouts = {}
+
+
+def _packed(device, *shapes):
+    """Uninitialised int32 tensors of these shapes in one allocation, each on a 16-byte boundary. (An allocation of its own for each
+    takes the host two to four times as long, which is what the small kernels behind it wait for.)"""
+    layout = _layouts.get(shapes)
+    if layout is None:
+        views, at = [], 0
+        for shape in shapes:
+            strides, words = [], 1
+            for n in reversed(shape):
+                strides.insert(0, words)
+                words *= n
+            views.append((shape, tuple(strides), at))
+            at += (words + 3) // 4 * 4
+        if len(_layouts) >= 4096:
+            _layouts.clear()
+        layout = _layouts[shapes] = (views, at)
+    buf = torch.empty(layout[1], dtype=torch.int32, device=device)
+    return [buf.as_strided(*view) for view in layout[0]]
 
 
 def verify_drafts(logits: torch.Tensor, token_ids: torch.Tensor, cu_rows: torch.Tensor, *, max_drafts: int,
@@ -2455,14 +2479,14 @@ def verify_drafts(logits: torch.Tensor, token_ids: torch.Tensor, cu_rows: torch.
         if d == 0:
             draft_logits = None
     _on_current(device)
-    out = VerifiedDrafts(torch.empty((s, d + 1), dtype=torch.int32, device=device), torch.empty((s,), dtype=torch.int32, device=device),
-                         torch.empty((s, d), dtype=torch.float32, device=device))
+    tokens, counts, accept = _packed(device, (s, d + 1), (s,), (s, d))
+    accept = accept.view(torch.float32)
     # scratch of the call's own: calls on several streams, or in several captured graphs, do not meet in it
-    scratch = torch.empty((_verify_scratch_words(s, d, vocab, given > 0, draft_logits is not None),), dtype=torch.int32, device=device)
-    _run("drafts", "ti_verify_drafts", out.tokens.data_ptr(), out.counts.data_ptr(), out.accept.data_ptr(), logits.data_ptr(),
-         token_ids.data_ptr(), cu_rows.data_ptr(), n, vocab, s, d, *(_ptr(t) for t in options), _ptr(draft_logits), stride_s, stride_d,
+    scratch = torch.empty(_verify_scratch_words(s, d, vocab, given > 0, draft_logits is not None), dtype=torch.int32, device=device)
+    _run("drafts", "ti_verify_drafts", tokens.data_ptr(), counts.data_ptr(), accept.data_ptr(), logits.data_ptr(),
+         token_ids.data_ptr(), cu_rows.data_ptr(), n, vocab, s, d, *[_ptr(t) for t in options], _ptr(draft_logits), stride_s, stride_d,
          scratch.data_ptr(), _stream())
-    return out
+    return VerifiedDrafts(tokens, counts, accept)
 
 
 def _verify_scratch_words(*key) -> int:
@@ -2494,7 +2518,8 @@ def ngram_drafts(history: torch.Tensor, lengths: torch.Tensor, *, max_drafts: in
     device = history.device
     _check(lengths, "lengths", torch.int32, 1)
     s, d = lengths.shape[0], int(max_drafts)
-    _per_request(s, device, lengths=(lengths, torch.int32))
+    if lengths.device != device:
+        raise KernelError(f"ngram_drafts: the lengths lie on {lengths.device}, the history on {device}")
     if not 0 <= d <= MAX_DRAFTS:
         raise KernelError(f"ngram_drafts: max_drafts must be 0 to {MAX_DRAFTS}, got {d}")
     if not 1 <= min_match <= max_match <= 32:
@@ -2507,12 +2532,13 @@ def ngram_drafts(history: torch.Tensor, lengths: torch.Tensor, *, max_drafts: in
         _check(tokens, "tokens", torch.int32, 2)
         if tokens.shape[0] != s or tokens.shape[1] > 512 or tokens.device != device:
             raise KernelError(f"ngram_drafts: tokens must be [{s}, at most 512] on {device}, got {tuple(tokens.shape)} on {tokens.device}")
-    optional = dict(counts=counts, state_slots=state_slots, limits=limits)
-    _per_request(s, device, **{name: (t, torch.int32) for name, t in optional.items() if t is not None})
+    for name, t in (("counts", counts), ("state_slots", state_slots), ("limits", limits)):
+        if t is not None:
+            _per_request(s, device, **{name: (t, torch.int32)})
     if status is not None:
         _check(status, "status", torch.int32, 1)
     _on_current(device)
-    out = NgramDrafts(torch.empty((s, d + 1), dtype=torch.int32, device=device), *torch.empty((3, s), dtype=torch.int32, device=device))
+    out = NgramDrafts(*_packed(device, (s, d + 1), (s,), (s,), (s,)))
     _run("drafts", "ti_ngram_drafts", out.tokens.data_ptr(), out.counts.data_ptr(), out.starts.data_ptr(), out.lengths.data_ptr(),
          history.data_ptr(), lengths.data_ptr(), _ptr(state_slots), _ptr(tokens), _ptr(counts), _ptr(limits), _ptr(status), s,
          history.shape[0], history.shape[1], tokens.shape[1] if tokens is not None else 0, d, int(min_match), int(max_match), _stream())
@@ -2535,9 +2561,10 @@ def step_arrays(starts: torch.Tensor, counts: torch.Tensor, block_tables: torch.
 
     What does not fit into ``max_count`` or ``rows``, and a request whose row or start does not exist, is left out and sets the
     ``status`` word, as a token without a page does (``page_status``)."""
+    rows, max_count, page_size, pad_page = int(rows), int(max_count), int(page_size), int(pad_page)
     _check(starts, "starts", torch.int32, 1)
     s, device = starts.shape[0], starts.device
-    _per_request(s, device, starts=(starts, torch.int32), counts=(counts, torch.int32))
+    _per_request(s, device, counts=(counts, torch.int32))
     if state_slots is not None:
         _per_request(s, device, state_slots=(state_slots, torch.int32))
     if block_tables.dim() == 2:
@@ -2560,20 +2587,15 @@ def step_arrays(starts: torch.Tensor, counts: torch.Tensor, block_tables: torch.
         _check(status, "status", torch.int32, 1)
     _on_current(device)
     tiles = s * -(-max_count // STEP_TILE)
-    sizes = [4 * tiles, groups * (s + 1) * width, groups * rows, rows, rows, rows if tokens is not None else 0, s + 2, s + 1, s + 1]
-    starts_at, total = [], 0
-    for words in sizes:                                  # one allocation; every array starts on a 16-byte boundary
-        starts_at.append(total)
-        total += (words + 3) // 4 * 4
-    buf = torch.empty((total,), dtype=torch.int32, device=device)
-    tile_v, table_v, slot_v, pos_v, seq_v, id_v, cu_v, start_v, ctx_v = (buf[at:at + words] for at, words in zip(starts_at, sizes))
-    out = StepArrays(id_v if tokens is not None else None, pos_v, seq_v, slot_v.view(groups, rows), cu_v, start_v, ctx_v,
-                     tile_v.view(tiles, 4), table_v.view(groups, s + 1, width))
-    _run("drafts", "ti_step_arrays", _ptr(out.token_ids), pos_v.data_ptr(), seq_v.data_ptr(), slot_v.data_ptr(), cu_v.data_ptr(),
-         start_v.data_ptr(), ctx_v.data_ptr(), tile_v.data_ptr(), table_v.data_ptr(), starts.data_ptr(), counts.data_ptr(),
-         _ptr(state_slots), block_tables.data_ptr(), _ptr(tokens), _ptr(status), s, groups, table_rows, width,
-         tokens.shape[1] if tokens is not None else 0, int(rows), int(max_count), int(page_size), int(pad_page), _stream())
-    return out
+    pos, seq, slots, cu, q_starts, ends, tile, table, *ids = _packed(
+        device, (rows,), (rows,), (groups, rows), (s + 2,), (s + 1,), (s + 1,), (tiles, 4), (groups, s + 1, width),
+        *([(rows,)] if tokens is not None else []))
+    flat = ids[0] if ids else None
+    _run("drafts", "ti_step_arrays", _ptr(flat), pos.data_ptr(), seq.data_ptr(), slots.data_ptr(), cu.data_ptr(), q_starts.data_ptr(),
+         ends.data_ptr(), tile.data_ptr(), table.data_ptr(), starts.data_ptr(), counts.data_ptr(), _ptr(state_slots),
+         block_tables.data_ptr(), _ptr(tokens), _ptr(status), s, groups, table_rows, width, tokens.shape[1] if tokens is not None else 0,
+         rows, max_count, page_size, pad_page, _stream())
+    return StepArrays(flat, pos, seq, slots, cu, q_starts, ends, tile, table)
 
 
 STEP_TILE = 128           # query rows of the tiles that step_arrays makes: the one-tile attention kernels'
