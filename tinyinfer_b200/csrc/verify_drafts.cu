@@ -16,14 +16,18 @@
 //
 // Bound by reading the logits once. Three kernels:
 //   parts_kernel   streams every row, 32 logits a thread in registers, and leaves of each warp's part the largest, the sum and the best
-//                  draw, or of a top-k row each THREAD's largest logit (a 32nd of the row); no block waits for another, no warp for another.
-//   rows_kernel    a block a row. Of a top-k row: at least k of 256 of these largest logits reach a value close to the k-th largest
-//                  of the 256, which bounds the row's k-th largest from below; so the row's top k are in the few threads' parts (some
-//                  110 for k = 100) that reach it, and those are read again and ranked.
+//                  draw, or of a top-k row the largest of every 32 neighbouring logits; no block waits for another, no warp for another.
+//   rows_kernel    a block a row. Of a top-k row: at least k of the row's lines of 32 reach a value close to the k-th largest of its lines'
+//                  largest, which bounds the row's k-th largest from below; so the row's top k are in the few lines (some 110 for k = 100)
+//                  that reach it, and those are read again and ranked.
 //   verify_kernel  decides the request; behind a drawn draft that failed, clusters of blocks scan the two rows once more.
+// The last two are short: most of their time is the wait for their own instructions (a line of eight that no block of the SM has run yet
+// costs some 240 cycles), so their loops are rolled and what is used twice is a function.
 // A row held by a cluster of 16 blocks in shared memory, threshold and sum found there, read the logits once too, but spent 13 us of a
 // block on meeting the others (a cluster's barrier 0.9 us) where its loads took 1.3: 291 us for 64 x 4 rows of 151,936 with k = 100.
 #include <cooperative_groups.h>
+
+#include <algorithm>
 
 #include "draws.cuh"
 
@@ -36,11 +40,12 @@ constexpr int VD_THREADS = 256;
 constexpr int VD_WARPS = VD_THREADS / 32;
 constexpr int VD_GROUPS = 8;         // groups of four logits a thread holds
 constexpr int VD_TILE = VD_THREADS * VD_GROUPS * 4;
-constexpr int VD_CANDIDATES = 3584;  // of a top-k row, in shared memory (14 a thread)
+constexpr int VD_LINE = 32;          // neighbouring logits that a top-k row's largest are taken of
+constexpr int VD_CANDIDATES = 2048;  // of a top-k row, in shared memory
 constexpr int VD_MAX_VOCAB = 1 << 19;        // so many weights of at most 2^44 fit 64 bits
 constexpr int VD_LIST = 256;         // of what the threshold keeps, for the draw behind a draft that failed
 constexpr int VD_CTAS = 8;           // blocks that share such a draw
-constexpr int VD_SCAN = 4;           // groups of four tokens a thread takes at a time there
+constexpr int VD_STAGES = 6;         // groups of four tokens on their way to a thread there
 constexpr float LOG2E = 1.4426950408889634f;
 
 // A warp's part of a row: the largest scaled logit, the sum of the exponentials relative to it, the best draw.
@@ -60,7 +65,7 @@ struct VdArgs {
     const int *stream_id, *step;
     const float* draft_logits;       // element (r, j, i) at r * draft_request + j * draft_place + i, or null
     long long draft_request, draft_place;
-    float* parts;                    // [requests, places, tiles, VD_THREADS]: threads' largest logits, or warps' Parts
+    float* parts;                    // [requests, places, tiles, VD_THREADS]: lines' largest logits, or warps' Parts
     RowStats* stats;                 // [requests, places], where not all are greedy
     Kept* kept;                      // [requests, max_drafts, VD_LIST]
     int* tokens;                     // [requests, max_drafts + 1]
@@ -157,8 +162,8 @@ __device__ __forceinline__ void load_four(const float* x, int e, int vocab, int 
     }
 }
 
-// The tokens of thread t in a tile: groups of four, VD_THREADS groups apart.
-__device__ __forceinline__ int token_of(int tile, int t, int k) { return tile * VD_TILE + 4 * (t + k * VD_THREADS); }
+// The tokens of thread t in a tile: a warp has 32 lines, a lane a group of four of every fourth.
+__device__ __forceinline__ int token_of(int tile, int t, int k) { return tile * VD_TILE + (t >> 5) * (32 * VD_LINE) + 4 * (32 * k + (t & 31)); }
 
 // DRAWS: open rows draw here, too (drafts that nothing judges: every row's token is wanted).
 template <bool DRAWS>
@@ -176,7 +181,7 @@ __global__ void __launch_bounds__(VD_THREADS, DRAWS ? 4 : 5) parts_kernel(VdArgs
         const float4* from = reinterpret_cast<const float4*>(at.x + token_of(blockIdx.x, tid, 0));
 #pragma unroll
         for (int k = 0; k < VD_GROUPS; ++k) {
-            const float4 f = from[k * VD_THREADS];
+            const float4 f = from[k * 32];
             v[k][0] = f.x; v[k][1] = f.y; v[k][2] = f.z; v[k][3] = f.w;
         }
     } else {
@@ -197,18 +202,31 @@ __global__ void __launch_bounds__(VD_THREADS, DRAWS ? 4 : 5) parts_kernel(VdArgs
         if (lane == 0) *part = Part{0.f, 0.f, b.v, b.i};
         return;
     }
-    float most = -INFINITY;
 #pragma unroll
     for (int k = 0; k < VD_GROUPS; ++k)
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            v[k][q] = fmaxf(v[k][q], -INFINITY);             // NaN, and what lies behind the row: -inf
-            most = fmaxf(most, v[k][q]);
-        }
+        for (int q = 0; q < 4; ++q) v[k][q] = fmaxf(v[k][q], -INFINITY);         // NaN, and what lies behind the row: -inf
     if (has_threshold(a.topk[r], a.vocab)) {
-        out[tid] = most;
+        // Eight neighbouring lanes share a line in each of their groups: after three exchanges, of four, two and one of the groups'
+        // largest, each of the eight has one line's, group lane % 8's.
+        float m[VD_GROUPS];
+#pragma unroll
+        for (int k = 0; k < VD_GROUPS; ++k) m[k] = fmaxf(fmaxf(v[k][0], v[k][1]), fmaxf(v[k][2], v[k][3]));
+#pragma unroll
+        for (int half = VD_GROUPS / 2; half > 0; half >>= 1) {
+            const bool upper = lane & half;
+#pragma unroll
+            for (int k = 0; k < half; ++k) {
+                const float other = __shfl_xor_sync(~0u, upper ? m[k] : m[k + half], half);
+                m[k] = fmaxf(upper ? m[k + half] : m[k], other);
+            }
+        }
+        out[(tid & ~31) + 4 * (lane & 7) + (lane >> 3)] = m[0];
         return;
     }
+    float most = -INFINITY;
+#pragma unroll
+    for (int k = 0; k < VD_GROUPS; ++k) most = fmaxf(most, fmaxf(fmaxf(v[k][0], v[k][1]), fmaxf(v[k][2], v[k][3])));
     const float temp = a.temperature[r], m = warp_max(most) / temp;
     const Weights weight(temp, m);
     float z = 0.f;
@@ -298,102 +316,114 @@ __device__ __forceinline__ RowStats whole_row(const VdArgs& a, const Place& at, 
 }
 
 struct RowShared {
-    float most[VD_THREADS];
-    alignas(16) unsigned key[VD_CANDIDATES];                  // read four at a time
+    unsigned key[VD_CANDIDATES];
     int idx[VD_CANDIDATES];
-    int part[VD_CANDIDATES];         // the threads' parts that hold candidates
-    unsigned hist[256], sel[2];
+    int line[VD_CANDIDATES];         // the lines that hold candidates
+    unsigned hist[256], sel[2], top[VD_WARPS];
     float red[33];
     Best best[VD_WARPS];
     unsigned long long total[VD_WARPS];
-    int parts, count, listed;
+    int lines, count, listed;
 };
-
-// The threads' largest logits of a row, number i of n at thread i % VD_THREADS: the first VD_KEPT of a thread in registers (rows of up to
-// 163,840 tokens have no more), the others read where they are wanted.
-constexpr int VD_KEPT = 20;
-struct Largest {
-    const float* of;
-    int n;
-    float kept[VD_KEPT];
-    __device__ __forceinline__ Largest(const float* of_, int n_) : of(of_), n(n_) {
-#pragma unroll
-        for (int k = 0; k < VD_KEPT; ++k) {
-            const int i = (int)threadIdx.x + k * VD_THREADS;
-            kept[k] = i < n ? of[i] : -INFINITY;
-        }
-    }
-    template <typename F> __device__ __forceinline__ void each(F f) const {
-#pragma unroll
-        for (int k = 0; k < VD_KEPT; ++k) f(kept[k]);
-        for (int i = (int)threadIdx.x + VD_KEPT * VD_THREADS; i < n; i += VD_THREADS) f(of[i]);
-    }
-};
-
-// A value that at least k of the threads' largest logits reach; -inf if there is none.
-__device__ __forceinline__ float top_bound(RowShared& sh, const Largest& largest, int k) {
-    const int tid = threadIdx.x, lane = tid & 31;
-    if (k > largest.n) return -INFINITY;
-    if (k <= VD_THREADS) {
-        // Every thread takes the largest of its own; a value near the k-th largest of these 256 (at least k reach it, an eighth more at
-        // most unless they are equal) by halving, every warp for itself: 8 keys a lane and one addition over the warp a step. (Counting for each
-        // of the 256 how many pass it: 2,000 cycles; these steps: 500.)
-        float own = -INFINITY;
-        largest.each([&](float v) { own = fmaxf(own, v); });
-        sh.most[tid] = own;
-        __syncthreads();
-        unsigned key[VD_WARPS], lo = ~0u, hi = 0u;
-#pragma unroll
-        for (int i = 0; i < VD_WARPS; ++i) {
-            key[i] = order_key(sh.most[lane + 32 * i]);
-            lo = min(lo, key[i]);
-            hi = max(hi, key[i]);
-        }
-        lo = __reduce_min_sync(~0u, lo);
-        hi = __reduce_max_sync(~0u, hi);
-        for (int reach = VD_THREADS; lo < hi && reach > k + k / 8;) {
-            const unsigned middle = lo + (hi - lo + 1) / 2;
-            int mine = 0;
-#pragma unroll
-            for (int i = 0; i < VD_WARPS; ++i) mine += key[i] >= middle;
-            mine = __reduce_add_sync(~0u, mine);
-            if (mine >= k) { lo = middle; reach = mine; }
-            else hi = middle - 1;
-        }
-        return key_value(lo);
-    }
-    unsigned lo = order_key(-INFINITY), hi = order_key(INFINITY);     // at least k reach lo
-    for (int i = 0; i < 20 && lo < hi; ++i) {
-        const unsigned middle = lo + (hi - lo + 1) / 2;
-        int reach = 0;
-        largest.each([&](float v) { reach += order_key(v) >= middle; });
-        reach = (int)block_sum((float)reach, sh.red);                 // at most 2^14 of them: exact
-        if (reach >= k) lo = middle;
-        else hi = middle - 1;
-    }
-    return key_value(lo);
-}
 
 // Places in a shared list for the bits that a thread has set in `mask`: the first one's (a warp asks for all of its own at once).
-__device__ __forceinline__ int places_for(unsigned mask, int* counter) {
+__device__ __noinline__ int places_for(unsigned mask, int* counter) {
     const int lane = threadIdx.x & 31, n = __popc(mask);
-    int upto = n;
+    int upto = n, base = 0;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
         const int w = __shfl_up_sync(~0u, upto, o);
         if (lane >= o) upto += w;
     }
-    int base = 0;
     if (lane == 31 && upto > 0) base = atomicAdd(counter, upto);
     return __shfl_sync(~0u, base, 31) + upto - n;
 }
 
+// The largest of the block's keys, two a thread.
+__device__ __noinline__ unsigned largest_key(unsigned one, unsigned two, unsigned* top_sh) {
+    const unsigned own = __reduce_max_sync(~0u, max(one, two));
+    if ((threadIdx.x & 31) == 0) top_sh[threadIdx.x >> 5] = own;
+    __syncthreads();
+    return __reduce_max_sync(~0u, top_sh[threadIdx.x & (VD_WARPS - 1)]);
+}
+
+// Of up to 512 keys, two a thread (0 where a thread has none; pairs: not all of the second are), of which at least k reach lo and none
+// passes hi: a value that at least k reach, and no more than k + spare unless they are equal, by halving; a step is a count over the block.
+__device__ __noinline__ unsigned reached_by(unsigned one, unsigned two, bool pairs, unsigned lo, unsigned hi, int k, int spare) {
+#pragma unroll 1
+    while (lo < hi) {
+        const unsigned middle = lo + (hi - lo + 1) / 2;
+        int n = __syncthreads_count(one >= middle);
+        if (pairs) n += __syncthreads_count(two >= middle);
+        if (n < k) {
+            hi = middle - 1;
+        } else {
+            lo = middle;
+            if (n <= k + spare) break;
+        }
+    }
+    return lo;
+}
+
+// The same for any number of lines, by halving over all of them: a k in the hundreds.
+__device__ __noinline__ unsigned lines_reached_by(RowShared& sh, const float* largest, int n, int k) {
+    unsigned lo = order_key(-INFINITY), hi = order_key(INFINITY);     // at least k reach lo
+#pragma unroll 1
+    for (int i = 0; i < 20 && lo < hi; ++i) {
+        const unsigned middle = lo + (hi - lo + 1) / 2;
+        int reach = 0;
+        for (int j = threadIdx.x; j < n; j += VD_THREADS) reach += order_key(largest[j]) >= middle;
+        reach = (int)block_sum((float)reach, sh.red);                 // at most 2^14 of them: exact
+        if (reach >= k) lo = middle;
+        else hi = middle - 1;
+    }
+    return lo;
+}
+
+// Copies four neighbouring logits (NaN behind the row's end) to shared memory, for the thread that asks.
+__device__ __forceinline__ void copy_four(float* to, const float* x, int e, int vocab, int step) {
+    const uint32_t d = (uint32_t)__cvta_generic_to_shared(to);
+    const float* from = x + e;
+    if (step == 4 && e + 3 < vocab) {
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(d), "l"(from) : "memory");
+    } else if (step == 2 && e + 3 < vocab) {
+        asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(d), "l"(from) : "memory");
+        asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(d + 8), "l"(from + 2) : "memory");
+    } else {
+#pragma unroll 1
+        for (int j = 0; j < 4; ++j) {
+            if (e + j < vocab) asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(d + 4 * j), "l"(from + j) : "memory");
+            else to[j] = NAN;
+        }
+    }
+}
+
+// s + G of token i, and the share's time in the race: both are functions, there is one copy of their logarithms.
+__device__ __noinline__ float exponential_of(int i, unsigned c1, unsigned stream, unsigned domain, uint2 key2) {
+    uint4 c = make_uint4((unsigned)i >> 2, c1, stream, domain);
+#pragma unroll 1
+    for (int round = 0; round < 10; ++round) {
+        c = philox_round(c, key2);
+        key2.x += 0x9E3779B9u;
+        key2.y += 0xBB67AE85u;
+    }
+    return -logf(philox_uniform(word_of(c, i)));
+}
+
+// Which of four logits reach `low`, as bits.
+__device__ __forceinline__ unsigned reach_of(float4 f, float low) {
+    auto bit = [&](float v, unsigned which) { return v >= low && v > -INFINITY ? which : 0u; };
+    return bit(f.x, 1u) | bit(f.y, 2u) | bit(f.z, 4u) | bit(f.w, 8u);
+}
+
+constexpr int VD_STAGED = 16384;     // bytes of lines read again at a time, at least
+
 __global__ void __launch_bounds__(VD_THREADS, 4) rows_kernel(VdArgs a) {
+    extern __shared__ __align__(16) float largest[];         // the lines' largest, then lines
     __shared__ RowShared sh;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, r = blockIdx.y, D = a.max_drafts;
     ti_grid_launch_dependents();
-    if (tid == 0) sh.parts = sh.count = sh.listed = 0;
-    __syncthreads();
+    if (tid == 0) sh.lines = sh.count = sh.listed = 0;
     ti_grid_wait();
     const int2 rows = rows_of(a, r);
     const bool greedy = is_greedy(a, r);
@@ -409,161 +439,136 @@ __global__ void __launch_bounds__(VD_THREADS, 4) rows_kernel(VdArgs a) {
         if (lane == 0) a.stats[slot] = st;
         return;
     }
-    const Largest largest(a.parts + slot * a.tiles * VD_THREADS, a.tiles * VD_THREADS);
+    const int n_lines = a.tiles * VD_THREADS, step = row_step(at.x);
+    const float* left = a.parts + slot * a.tiles * VD_THREADS;
+#pragma unroll 1
+    for (int i = 4 * tid; i < n_lines; i += 4 * VD_THREADS) copy_four(largest + i, left, i, n_lines, 4);
     const float at_draft = drafted >= 0 && drafted < a.vocab ? at.x[drafted] : NAN;
-    const uint2 key2 = at.draws ? seed_of(a, r) : make_uint2(0u, 0u);
-    const unsigned c1 = at.draws ? (unsigned)(a.step[r] + at.j) : 0u, stream = at.draws ? (unsigned)a.stream_id[r] : 0u;
-    const int step = row_step(at.x);
-    const bool lists = !at.draws && (int)blockIdx.x <= D;             // a draw behind a failed draft may want them
-    Kept* kept = lists ? a.kept + ((size_t)r * D + at.j) * VD_LIST : nullptr;
+    const bool lists = !at.draws && (int)blockIdx.x <= D;    // a draw behind a failed draft may want them
     RowStats st{0.f, 0.f, 0u, -1, 0.f, -1, {0, 0}};
-    unsigned long long sum = 0;                                       // weights of at most 1 in steps of 2^-44
+    unsigned long long sum = 0;                              // weights of at most 1 in steps of 2^-44
     Best b{0.f, -1};
+    unsigned top;
+    asm volatile("cp.async.wait_all;" ::: "memory");
 
-    const float low = below_quotient(top_bound(sh, largest, topk), temp);
-    {
+    __syncthreads();
+
+    // A value that k lines' largest reach: by the largest of two shares of a thread's lines if those are enough, otherwise by all.
+    float one = -INFINITY, two = -INFINITY;
+#pragma unroll 2
+    for (int i = tid; i < n_lines; i += 2 * VD_THREADS) {
+        one = fmaxf(one, largest[i]);
+        if (i + VD_THREADS < n_lines) two = fmaxf(two, largest[i + VD_THREADS]);
+    }
+    top = largest_key(order_key(one), order_key(two), sh.top);
+    const unsigned bound = topk <= 2 * VD_THREADS ? reached_by(order_key(one), order_key(two), true, order_key(-INFINITY), top, topk, topk / 8)
+                                                  : lines_reached_by(sh, largest, n_lines, topk);
+    const float reached = key_value(bound), low = below_quotient(reached, temp);
+    constexpr int FOURS = 5;                                 // groups of four a thread looks at together
+#pragma unroll 1
+    for (int first = 0; first < n_lines; first += FOURS * 4 * VD_THREADS) {
         unsigned hits = 0u;
 #pragma unroll
-        for (int k = 0; k < VD_KEPT; ++k) hits |= largest.kept[k] >= low && largest.kept[k] > -INFINITY ? 1u << k : 0u;
-        int to = places_for(hits, &sh.parts);
-#pragma unroll
-        for (int k = 0; k < VD_KEPT; ++k)
-            if (hits >> k & 1u) {
-                if (to < VD_CANDIDATES) sh.part[to] = tid + k * VD_THREADS;
-                ++to;
-            }
-        for (int i = tid + VD_KEPT * VD_THREADS; i < largest.n; i += VD_THREADS)
-            if (largest.of[i] >= low && largest.of[i] > -INFINITY) {
-                to = atomicAdd(&sh.parts, 1);
-                if (to < VD_CANDIDATES) sh.part[to] = i;
-            }
+        for (int k = 0; k < FOURS; ++k) {
+            const int i = first + 4 * (k * VD_THREADS + tid);
+            if (i < n_lines) hits |= reach_of(*reinterpret_cast<const float4*>(largest + i), low) << (4 * k);
+        }
+        int to = places_for(hits, &sh.lines);
+        for (; hits; hits &= hits - 1u, ++to) {
+            const int bit = __ffs(hits) - 1;
+            if (to < VD_CANDIDATES) sh.line[to] = first + 4 * ((bit >> 2) * VD_THREADS + tid) + (bit & 3);
+        }
     }
     __syncthreads();
-    const int n_groups = sh.parts * VD_GROUPS;
-    bool fits = sh.parts <= VD_CANDIDATES;
+    bool fits = sh.lines <= VD_CANDIDATES;
     if (fits) {
-        // their logits once more, a thread a group, four in flight
-        for (int first = 0; first < n_groups; first += 4 * VD_THREADS) {
-            float v[4][4];
-            int e[4];
+        // their logits once more, a lane a group, as many lines at a time as there is room for where the largest were
+        const int groups = sh.lines * (VD_LINE / 4), room = max(n_lines * 4, VD_STAGED) / 16;
+        auto token = [&](int g) { return sh.line[g / (VD_LINE / 4)] * VD_LINE + g % (VD_LINE / 4) * 4; };
+#pragma unroll 1
+        for (int first = 0; first < groups; first += room) {
+            const int some = min(room, groups - first);
+            // (a thread copies, reads and copies over its own groups only)
+#pragma unroll 1
+            for (int g = tid; g < some; g += VD_THREADS) copy_four(largest + 4 * g, at.x, token(first + g), a.vocab, step);
+            asm volatile("cp.async.wait_all;" ::: "memory");
+#pragma unroll 1
+            for (int base = 0; base < some; base += FOURS * VD_THREADS) {
+                unsigned hits = 0u;
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const int w = first + k * VD_THREADS + tid;
-                e[k] = a.vocab;
-                if (w < n_groups) {
-                    const int i = sh.part[w / VD_GROUPS];
-                    e[k] = token_of(i / VD_THREADS, i % VD_THREADS, w % VD_GROUPS);
+                for (int k = 0; k < FOURS; ++k) {
+                    const int g = base + k * VD_THREADS + tid;
+                    if (g < some) hits |= reach_of(*reinterpret_cast<const float4*>(largest + 4 * g), low) << (4 * k);
                 }
-                load_four(at.x, e[k], a.vocab, step, v[k]);
-            }
-            unsigned hits = 0u;
-#pragma unroll
-            for (int k = 0; k < 4; ++k)
-#pragma unroll
-                for (int q = 0; q < 4; ++q) hits |= v[k][q] >= low && v[k][q] > -INFINITY ? 1u << (4 * k + q) : 0u;
-            int to = places_for(hits, &sh.count);
-#pragma unroll
-            for (int k = 0; k < 4; ++k)
-#pragma unroll
-                for (int q = 0; q < 4; ++q)
-                    if (hits >> (4 * k + q) & 1u) {
-                        if (to < VD_CANDIDATES) {
-                            sh.key[to] = __float_as_uint(v[k][q]);
-                            sh.idx[to] = e[k] + q;
-                        }
-                        ++to;
+                int to = places_for(hits, &sh.count);
+                for (; hits; hits &= hits - 1u, ++to) {
+                    const int bit = __ffs(hits) - 1, g = base + (bit >> 2) * VD_THREADS + tid;
+                    if (to < VD_CANDIDATES) {
+                        sh.key[to] = score_key(largest[4 * g + (bit & 3)] / temp);
+                        sh.idx[to] = token(first + g) + (bit & 3);
                     }
+                }
+            }
         }
         __syncthreads();
         fits = sh.count <= VD_CANDIDATES;
     }
-    if (fits) {
-        const int n = sh.count;
-        for (int i = tid; i < n; i += VD_THREADS) sh.key[i] = score_key(__uint_as_float(sh.key[i]) / temp);
-        if (tid < 4 && n + tid < VD_CANDIDATES) sh.key[n + tid] = 0u;         // (no key of a number is 0)
-        if (tid == 0) sh.sel[0] = sh.sel[1] = 0u;
-        __syncthreads();
-        if (n <= 2 * VD_THREADS) {
-            // the k-th largest is the key that fewer than k pass and with its equals k reach; fewer than k in all: no finite logit of
-            // the row is missing, and all are kept
-            const uint4* keys = reinterpret_cast<const uint4*>(sh.key);
-            for (int i = tid; i < n; i += VD_THREADS) {
-                const unsigned own = sh.key[i];
-                int above = 0, level = 0;
-#pragma unroll 4
-                for (int o = 0; o < (n + 3) / 4; ++o) {
-                    const uint4 k4 = keys[o];
-                    above += (k4.x > own) + (k4.y > own) + (k4.z > own) + (k4.w > own);
-                    level += (k4.x == own) + (k4.y == own) + (k4.z == own) + (k4.w == own);
-                }
-                if (above < topk && topk <= above + level) sh.sel[0] = own;
-                if (above == 0) sh.sel[1] = own;
-            }
-            __syncthreads();
-            st.threshold = sh.sel[0];
-            st.m = n > 0 ? key_value(sh.sel[1]) : -INFINITY;
-        } else {
-            if (n >= topk)
-                st.threshold = select_kth(topk, sh.hist, sh.sel, [&](auto count) {
-                    for (int i = tid; i < n; i += VD_THREADS) count(sh.key[i]);
-                });
-            float top = -INFINITY;
-            for (int i = tid; i < n; i += VD_THREADS) top = fmaxf(top, key_value(sh.key[i]));
-            st.m = block_max(top, sh.red);
-        }
-        for (int i = tid; i < n; i += VD_THREADS) {
-            if (sh.key[i] < st.threshold) continue;
-            const float s = key_value(sh.key[i]);
-            sum += __float2ull_rn(scaled_weight(s, st.m) * 17592186044416.f);
-            if (at.draws) {
-                const uint4 w = philox4x32_10(make_uint4((unsigned)sh.idx[i] >> 2, c1, stream, 0u), key2);
-                b = better(b, Best{noisy(s, philox_uniform(word_of(w, sh.idx[i]))), sh.idx[i]});
-            }
-            if (lists) {
-                const int to = atomicAdd(&sh.listed, 1);
-                if (to < VD_LIST) kept[to] = Kept{s, sh.idx[i]};
-            }
-        }
+    const uint2 key2 = at.draws ? seed_of(a, r) : make_uint2(0u, 0u);
+    const unsigned c1 = at.draws ? (unsigned)(a.step[r] + at.j) : 0u, stream = at.draws ? (unsigned)a.stream_id[r] : 0u;
+    Kept* kept = lists ? a.kept + ((size_t)r * D + at.j) * VD_LIST : nullptr;
+    const int n = fits ? sh.count : a.vocab;
+    if (fits && n <= 2 * VD_THREADS) {
+        // fewer than k: no finite logit of the row is missing, and all are kept
+        const unsigned first = tid < n ? sh.key[tid] : 0u, second = tid + VD_THREADS < n ? sh.key[tid + VD_THREADS] : 0u;
+        top = largest_key(first, second, sh.top);
+        if (n >= topk) st.threshold = reached_by(first, second, n > VD_THREADS, score_key(reached / temp), top, topk, 0);
+        st.m = n > 0 ? key_value(top) : -INFINITY;
     } else {
-        // More candidates than there is room for (a k in the thousands, thousands of equal logits): the row itself, pass by pass.
-        st.threshold = select_kth(topk, sh.hist, sh.sel, [&](auto count) {
-            for (int i = tid; i < a.vocab; i += VD_THREADS) {
-                const float s = at.x[i] / temp;
-                if (s == s) count(score_key(s));
-            }
-        });
-        float top = -INFINITY;
-        for (int i = tid; i < a.vocab; i += VD_THREADS) top = fmaxf(top, at.x[i] / temp);
-        st.m = block_max(top, sh.red);
-        for (int i = tid; i < a.vocab; i += VD_THREADS) {
-            const float s = at.x[i] / temp;
-            if (!(s > -INFINITY) || score_key(s) < st.threshold) continue;
-            sum += __float2ull_rn(scaled_weight(s, st.m) * 17592186044416.f);
-            if (at.draws) {
-                const uint4 w = philox4x32_10(make_uint4((unsigned)i >> 2, c1, stream, 0u), key2);
-                b = better(b, Best{noisy(s, philox_uniform(word_of(w, i))), i});
-            }
-        }
-        if (tid == 0) sh.listed = VD_LIST + 1;
+        // many candidates; or more than there is room for (a k in the thousands, thousands of equal logits): the row itself
+        auto scaled = [&](int i) { return fits ? key_value(sh.key[i]) : at.x[i] / temp; };
+        if (n >= topk)
+            st.threshold = select_kth(topk, sh.hist, sh.sel, [&](auto count) {
+                for (int i = tid; i < n; i += VD_THREADS) {
+                    const float s = scaled(i);
+                    if (s == s) count(score_key(s));
+                }
+            });
+        float largest_scaled = -INFINITY;
+        for (int i = tid; i < n; i += VD_THREADS) largest_scaled = fmaxf(largest_scaled, scaled(i));
+        st.m = block_max(largest_scaled, sh.red);
+        if (!fits && tid == 0) sh.listed = VD_LIST + 1;
     }
-#pragma unroll
+#pragma unroll 1
+    for (int i = tid; i < n; i += VD_THREADS) {
+        const float s = fits ? key_value(sh.key[i]) : at.x[i] / temp;
+        if (!(s > -INFINITY) || score_key(s) < st.threshold) continue;
+        const int token = fits ? sh.idx[i] : i;
+        sum += __float2ull_rn(scaled_weight(s, st.m) * 17592186044416.f);
+        if (at.draws) b = better(b, Best{s - logf(exponential_of(token, c1, stream, 0u, key2)), token});
+        if (lists && fits) {
+            const int to = atomicAdd(&sh.listed, 1);
+            if (to < VD_LIST) kept[to] = Kept{s, token};
+        }
+    }
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
     b = warp_best(b);
     if (lane == 0) { sh.total[warp] = sum; sh.best[warp] = b; }
     __syncthreads();
     if (warp > 0) return;
-    sum = lane < VD_WARPS ? sh.total[lane] : 0;
+    sum = sh.total[lane & (VD_WARPS - 1)];
+    b = sh.best[lane & (VD_WARPS - 1)];
 #pragma unroll
-    for (int o = VD_WARPS / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
-    b = warp_best(lane < VD_WARPS ? sh.best[lane] : Best{0.f, -1});
-    if (lane == 0) {
-        st.z = (float)((double)sum * (1.0 / 17592186044416.0));
-        st.drawn = b.i;
-        const float s = at_draft / temp;
-        if (s > -INFINITY && score_key(s) >= st.threshold) st.share = scaled_weight(s, st.m) / st.z;
-        if (lists && sh.listed <= VD_LIST) st.listed = sh.listed;
-        a.stats[slot] = st;
+    for (int o = VD_WARPS / 2; o > 0; o >>= 1) {
+        sum += __shfl_xor_sync(~0u, sum, o);
+        b = better(b, Best{__shfl_xor_sync(~0u, b.v, o), __shfl_xor_sync(~0u, b.i, o)});
     }
+    if (lane > 0) return;
+    st.z = (float)((double)sum * (1.0 / 17592186044416.0));
+    st.drawn = b.i;
+    const float s = at_draft / temp;
+    if (s > -INFINITY && score_key(s) >= st.threshold) st.share = scaled_weight(s, st.m) / st.z;
+    if (lists && sh.listed <= VD_LIST) st.listed = sh.listed;
+    a.stats[slot] = st;
 }
 
 // Decides the request by its rows; if a drawn draft failed, draws from what is left of p beyond q. JUDGED: a cluster of blocks a
@@ -631,12 +636,8 @@ __global__ void __launch_bounds__(VD_THREADS, 4) verify_kernel(VdArgs a) {
             auto p_of = [&](float v) { return v > -INFINITY && (!st.threshold || score_key(v / temp) >= st.threshold) ? pw(v) * pz : 0.f; };
             auto q_of = [&](float v) { return v > -INFINITY && (!ds.threshold || score_key(v / temp) >= ds.threshold) ? qw(v) * qz : 0.f; };
             // An exponential race, the largest share / E, E = -log U; in ti_sample's terms the largest s + G.
-            auto number = [&](int i) {
-                const uint4 w = philox4x32_10(make_uint4((unsigned)i >> 2, c1, stream, domain), key2);
-                return philox_uniform(word_of(w, i));
-            };
             auto race = [&](float share, int i) {
-                if (share > 0.f) b = better(b, Best{share / -logf(number(i)), i});
+                if (share > 0.f) b = better(b, Best{share / exponential_of(i, c1, stream, domain, key2), i});
             };
             b.i = -1;
             if (failed && st.listed >= 0) {                  // the threshold keeps few: the first block alone
@@ -646,68 +647,70 @@ __global__ void __launch_bounds__(VD_THREADS, 4) verify_kernel(VdArgs a) {
                 b = block_best(b, best_sh);
             } else {
                 cg::cluster_group cluster = cg::this_cluster();
-                const int groups = (a.vocab + 3) / 4, x_step = row_step(x), y_step = row_step(y);
-                // Logits of both rows that no threshold and no infinity cuts: a multiply-add and an exponential each. Otherwise, every
-                // token by p_of and q_of.
-                const bool plain = !st.threshold && !ds.threshold && !pw.odd && !(failed && qw.odd) && st.z > 0.f;
-                // Only tokens whose share can still pass the best B of the warp run: share / E > B needs 1 - U < share / B, and 1 - U is exact.
-                float spare = INFINITY;                      // 1 / B
-                for (int first = rank * VD_SCAN * VD_THREADS; first < groups; first += VD_CTAS * VD_SCAN * VD_THREADS) {
-                    const int at = 4 * (first + tid);        // token 4 * k + i of the thread: at + 4 * VD_THREADS * k + i
-                    float p[VD_SCAN][4], q[VD_SCAN][4], ahead = 0.f;
-#pragma unroll
-                    for (int k = 0; k < VD_SCAN; ++k) load_four(x, at + 4 * VD_THREADS * k, a.vocab, x_step, p[k]);
-                    if (failed) {
-#pragma unroll
-                        for (int k = 0; k < VD_SCAN; ++k) load_four(y, at + 4 * VD_THREADS * k, a.vocab, y_step, q[k]);
+                extern __shared__ __align__(16) float ring[];                  // [stage][row][thread][4]: a thread's own
+                const int groups = (a.vocab + 3) / 4, stride = VD_CTAS * VD_THREADS, x_step = row_step(x), y_step = row_step(y);
+                auto fetch = [&](int g, int stage) {
+                    if (g < groups) {
+                        copy_four(ring + ((stage * 2) * VD_THREADS + tid) * 4, x, 4 * g, a.vocab, x_step);
+                        if (failed) copy_four(ring + ((stage * 2 + 1) * VD_THREADS + tid) * 4, y, 4 * g, a.vocab, y_step);
                     }
+                    asm volatile("cp.async.commit_group;" ::: "memory");
+                };
+                // Logits that no threshold and no infinity cuts: a share is 2^(v c - m log2 e - log2 z). Otherwise by p_of and q_of.
+                const bool plain = !st.threshold && !ds.threshold && !pw.odd && !(failed && qw.odd) && st.z > 0.f;
+                const float p2 = pw.m2 + log2f(st.z), q2 = failed ? qw.m2 + log2f(ds.z) : INFINITY;
+                // Only tokens whose share can still pass the best B of the warp run: share / E > B needs 1 - U < share / B. 1 - U is
+                // (2^23 - 1 - word / 2^9) / 2^23 + 2^-24, exactly; the first summand is had from the word's bits.
+                float spare = INFINITY;                      // 1 / B
+#pragma unroll 1
+                for (int k = 0; k < VD_STAGES; ++k) fetch((rank + k * VD_CTAS) * VD_THREADS + tid, k);
+                int stage = 0;
+#pragma unroll 1
+                for (int g = rank * VD_THREADS + tid; g - tid < groups; g += stride) {
+                    asm volatile("cp.async.wait_group %0;" ::"n"(VD_STAGES - 1) : "memory");
+                    float p[4], ahead = 0.f;
+                    {
+                        const float4 f = *reinterpret_cast<const float4*>(ring + ((stage * 2) * VD_THREADS + tid) * 4);
+                        p[0] = f.x; p[1] = f.y; p[2] = f.z; p[3] = f.w;
+                        float4 o = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+                        if (failed) o = *reinterpret_cast<const float4*>(ring + ((stage * 2 + 1) * VD_THREADS + tid) * 4);
+                        const float q[4] = {o.x, o.y, o.z, o.w};
+                        if (plain) {
 #pragma unroll
-                    for (int k = 0; k < VD_SCAN; ++k)
+                            for (int i = 0; i < 4; ++i) p[i] = ex2(fmaf(fmaxf(p[i], -INFINITY), pw.c, -p2)) - ex2(fmaf(fmaxf(q[i], -INFINITY), pw.c, -q2));
+                        } else {
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            if (plain) {
-                                p[k][i] = pw.fast(fmaxf(p[k][i], -INFINITY)) * pz;
-                                if (failed) p[k][i] = fmaf(-qz, qw.fast(fmaxf(q[k][i], -INFINITY)), p[k][i]);
-                            } else {
-                                p[k][i] = p_of(p[k][i]);
-                                if (failed) p[k][i] -= q_of(q[k][i]);
-                            }
-                            ahead = fmaxf(ahead, p[k][i]);
+                            for (int i = 0; i < 4; ++i) p[i] = p_of(p[i]) - (failed ? q_of(q[i]) : 0.f);
                         }
-                    bool again = false;
-                    do {
-                        unsigned run = 0u;
-                        again = plain && spare == INFINITY;  // nothing to beat yet: the foremost of every thread, then all
-                        if (again || !plain) {
+                        if (g >= groups) p[0] = p[1] = p[2] = p[3] = 0.f;
 #pragma unroll
-                            for (int k = 0; k < VD_SCAN; ++k)
+                        for (int i = 0; i < 4; ++i) ahead = fmaxf(ahead, p[i]);
+                    }
+                    fetch(g + VD_STAGES * stride, stage);    // (what lay there is in registers)
+                    stage = stage + 1 < VD_STAGES ? stage + 1 : 0;
+                    unsigned run = 0u;
+                    if (spare == INFINITY || !plain) {       // nothing to beat yet: all of them
 #pragma unroll
-                                for (int i = 0; i < 4; ++i) run |= p[k][i] > 0.f && (p[k][i] == ahead || !plain) ? 1u << (4 * k + i) : 0u;
-                        } else if (ahead * spare > 5.9e-8f) {                // 1 - U is 2^-24 at least
+                        for (int i = 0; i < 4; ++i) run |= p[i] > 0.f ? 1u << i : 0u;
+                    } else if (ahead * spare > 5.9e-8f) {    // 1 - U is 2^-24 at least
+                        const uint4 w = philox4x32_10(make_uint4((unsigned)g, c1, stream, domain), key2);
+                        const unsigned words[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-                            for (int k = 0; k < VD_SCAN; ++k) {
-                                const uint4 w = philox4x32_10(make_uint4((unsigned)(at + 4 * VD_THREADS * k) >> 2, c1, stream, domain), key2);
-                                const unsigned words[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-                                for (int i = 0; i < 4; ++i) run |= 1.f - philox_uniform(words[i]) < p[k][i] * spare ? 1u << (4 * k + i) : 0u;
-                            }
-                        }
+                        for (int i = 0; i < 4; ++i)
+                            run |= 1.99999988f - __uint_as_float(0x3F800000u | words[i] >> 9) < fmaf(p[i], spare, -5.9604645e-8f) ? 1u << i : 0u;
+                    }
+                    if (__any_sync(~0u, run)) {
+#pragma unroll 1
                         for (; run; run &= run - 1u) {
-                            const int bit = __ffs(run) - 1, i = at + 4 * VD_THREADS * (bit >> 2) + (bit & 3);
-                            if (failed) {
-                                float share = 0.f;           // the register file has no subscripts
-#pragma unroll
-                                for (int o = 0; o < 4 * VD_SCAN; ++o) share = bit == o ? p[o >> 2][o & 3] : share;
-                                race(share, i);
-                            } else {
-                                b = better(b, Best{noisy(x[i] / temp, number(i)), i});
-                            }
+                            const int i = __ffs(run) - 1;
+                            if (failed) race(i & 2 ? (i & 1 ? p[3] : p[2]) : (i & 1 ? p[1] : p[0]), 4 * g + i);
+                            else b = better(b, Best{x[4 * g + i] / temp - logf(exponential_of(4 * g + i, c1, stream, domain, key2)), 4 * g + i});
                         }
-                        const float best = warp_max(b.i < 0 ? -INFINITY : b.v);
-                        if (best > -INFINITY) spare = pw.spare() * (failed ? 1.f / best : ex2((st.m - best) * LOG2E) * st.z);
-                        again = again && spare != INFINITY;
-                    } while (again);
+                        const unsigned best = __reduce_max_sync(~0u, b.i < 0 ? 0u : order_key(b.v));
+                        if (best) spare = pw.spare() * (failed ? 1.f / key_value(best) : ex2((st.m - key_value(best)) * LOG2E) * st.z);
+                    }
                 }
+                asm volatile("cp.async.wait_all;" ::: "memory");
                 b = block_best(b, best_sh);
                 cluster.sync();                              // every block runs
                 if (tid == 0) *cluster.map_shared_rank(&part_sh[rank], 0) = b;
@@ -763,10 +766,16 @@ TI_API int ti_verify_drafts(int* tokens, int* counts, float* accept, const float
     ti_launch(draft_logits || !temperature ? parts_kernel<false> : parts_kernel<true>, dim3(a.tiles, a.places, requests), VD_THREADS, 0, stream, a);
     TI_CHECK_LAUNCH("verify_drafts: parts");
     if (temperature) {
-        ti_launch(rows_kernel, dim3(a.places, requests), VD_THREADS, 0, stream, a);
+        const int shared = std::max(a.tiles * VD_THREADS * 4, VD_STAGED);
+        TI_REQUIRE(ti_allow_shared<rows_kernel>(shared) == cudaSuccess, "verify_drafts: %d bytes of shared memory are not to be had", shared);
+        ti_launch(rows_kernel, dim3(a.places, requests), VD_THREADS, shared, stream, a);
         TI_CHECK_LAUNCH("verify_drafts: rows");
     }
-    if (draft_logits) ti_launch_clusters(verify_kernel<true, false>, dim3(VD_CTAS, requests), VD_CTAS, VD_THREADS, 0, stream, a);
+    if (draft_logits) {
+        constexpr int shared = VD_STAGES * 2 * VD_THREADS * 16;
+        TI_REQUIRE((ti_allow_shared<verify_kernel<true, false>>(shared) == cudaSuccess), "verify_drafts: %d bytes of shared memory are not to be had", shared);
+        ti_launch_clusters(verify_kernel<true, false>, dim3(VD_CTAS, requests), VD_CTAS, VD_THREADS, shared, stream, a);
+    }
     else ti_launch(temperature ? verify_kernel<false, false> : verify_kernel<false, true>, dim3(1, requests), VD_THREADS, 0, stream, a);
     TI_CHECK_LAUNCH("verify_drafts");
     return 0;
