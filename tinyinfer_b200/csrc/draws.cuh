@@ -29,9 +29,9 @@ __device__ __forceinline__ unsigned order_key(float v) {           // larger flo
     return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
 }
 
-// Launches `kernel` on clusters of `ctas` blocks along x, otherwise as ti_launch does.
+// Launches `kernel` on clusters of `ctas` blocks along x; early: as ti_launch does, otherwise as ti_launch_alone.
 template <typename... KArgs, typename... Args>
-cudaError_t ti_launch_clusters(void (*kernel)(KArgs...), dim3 grid, int ctas, dim3 block, size_t smem, cudaStream_t stream, Args... args) {
+cudaError_t ti_launch_clusters(void (*kernel)(KArgs...), dim3 grid, int ctas, dim3 block, size_t smem, bool early, cudaStream_t stream, Args... args) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = grid;
     cfg.blockDim = block;
@@ -44,7 +44,7 @@ cudaError_t ti_launch_clusters(void (*kernel)(KArgs...), dim3 grid, int ctas, di
     attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = ti_pdl_enabled() ? 2 : 1;
+    cfg.numAttrs = early && ti_pdl_enabled() ? 2 : 1;
     return cudaLaunchKernelEx(&cfg, kernel, KArgs(args)...);
 }
 

@@ -42,10 +42,11 @@ __device__ __forceinline__ unsigned long long warp_max64(unsigned long long v) {
     return v;
 }
 
-__global__ void __launch_bounds__(NG_THREADS) ngram_kernel(NgArgs a) {
+__global__ void __launch_bounds__(NG_THREADS, 5) ngram_kernel(NgArgs a) {
     __shared__ unsigned long long best_sh[NG_WARPS], part_sh[NG_CTAS];
     __shared__ int last_sh[NG_MAX_MATCH];
     ti_grid_launch_dependents();
+    if (gridDim.x > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
     ti_grid_wait();
     const int r = blockIdx.y, rank = blockIdx.x, ctas = gridDim.x, tid = threadIdx.x, D = a.max_drafts;
     const int row = a.state_slots ? a.state_slots[r] : r;
@@ -58,41 +59,51 @@ __global__ void __launch_bounds__(NG_THREADS) ngram_kernel(NgArgs a) {
     const int n = fits ? held + brought : (known ? held : 0);
     const bool there = fits && n > 0;
     auto token = [&](int i) { return i < held ? h[i] : fresh[i - held]; };        // nobody waits for the new ones to be written
+    // tokens 0 .. end - 1 as they lie; group g has those from 4 g - shift on. What is wanted of the first groups is under way before it
+    // is known what they are compared with.
+    const int end = there ? min(held, n - 1) : 0, shift = (int)(((uintptr_t)h >> 2) & 3), groups = (end + shift + 3) >> 2;
+    int4 v[NG_LOADS];
+    auto load = [&](int first) {
+#pragma unroll
+        for (int k = 0; k < NG_LOADS; ++k) {
+            const int g = first + k * NG_THREADS, i = 4 * g - shift;
+            if (i >= 0 && i + 3 < end) {
+                v[k] = *reinterpret_cast<const int4*>(h + i);
+            } else {                                         // the text's ends, and behind them
+                v[k].x = i >= 0 && i < end ? h[i] : 0;
+                v[k].y = i + 1 >= 0 && i + 1 < end ? h[i + 1] : 0;
+                v[k].z = i + 2 >= 0 && i + 2 < end ? h[i + 2] : 0;
+                v[k].w = i + 3 >= 0 && i + 3 < end ? h[i + 3] : 0;
+            }
+        }
+    };
+    int first = rank * NG_LOADS * NG_THREADS + tid;
+    load(first);
     if (there && tid < a.max_match && tid < n) last_sh[tid] = token(n - 1 - tid);
     __syncthreads();
     unsigned long long best = 0;
-    if (there && n > 1) {
+    if (there) {
         const int last = last_sh[0];
         auto look = [&](int i, int value) {                  // the match that ends with token i
-            if (value != last) return;
+            if (value != last || i < 0 || i >= n - 1) return;
             int l = 1;
             while (l < a.max_match && l <= i && token(i - l) == last_sh[l]) ++l;
             const unsigned long long key = ((unsigned long long)l << 32) | (unsigned)(i + 1);
             if (l >= a.min_match && key > best) best = key;
         };
-        // tokens 0 .. end - 1 as they lie; group g has those from 4 g - shift on
-        const int end = min(held, n - 1), shift = (int)(((uintptr_t)h >> 2) & 3), groups = (end + shift + 3) >> 2;
-        const int4* from = reinterpret_cast<const int4*>(h - shift);
-        for (int first = rank * NG_LOADS * NG_THREADS + tid; first < groups; first += ctas * NG_LOADS * NG_THREADS) {
-            int4 v[NG_LOADS];
-#pragma unroll
-            for (int k = 0; k < NG_LOADS; ++k) {
-                const int g = first + k * NG_THREADS, i = 4 * g - shift;
-                if (i >= 0 && i + 3 < end) {
-                    v[k] = from[g];
-                } else {                                     // the text's ends, and behind them (a token that is not `last`)
-                    v[k].x = i >= 0 && i < end ? h[i] : ~last;
-                    v[k].y = i + 1 >= 0 && i + 1 < end ? h[i + 1] : ~last;
-                    v[k].z = i + 2 >= 0 && i + 2 < end ? h[i + 2] : ~last;
-                    v[k].w = i + 3 >= 0 && i + 3 < end ? h[i + 3] : ~last;
-                }
-            }
+        while (true) {
 #pragma unroll
             for (int k = 0; k < NG_LOADS; ++k) {
                 const int i = 4 * (first + k * NG_THREADS) - shift;
-                if (v[k].x != last && v[k].y != last && v[k].z != last && v[k].w != last) continue;
-                look(i, v[k].x); look(i + 1, v[k].y); look(i + 2, v[k].z); look(i + 3, v[k].w);
+                if (i >= end || (v[k].x != last && v[k].y != last && v[k].z != last && v[k].w != last)) continue;
+                const int token4[4] = {v[k].x, v[k].y, v[k].z, v[k].w};
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+                    if (i + q < end) look(i + q, token4[q]);
             }
+            first += ctas * NG_LOADS * NG_THREADS;
+            if (first >= groups) break;
+            load(first);
         }
         if (rank == 0)                                       // the new ones but the last
             for (int i = held + tid; i < n - 1; i += NG_THREADS) look(i, token(i));
@@ -103,7 +114,7 @@ __global__ void __launch_bounds__(NG_THREADS) ngram_kernel(NgArgs a) {
     best = warp_max64((tid & 31) < NG_WARPS ? best_sh[tid & 31] : 0ull);
     if (ctas > 1) {
         cg::cluster_group cluster = cg::this_cluster();
-        cluster.sync();                                      // every block runs
+        asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");           // every block runs
         if (tid == 0) *cluster.map_shared_rank(&part_sh[rank], 0) = best;
         cluster.sync();
         if (rank != 0) return;
@@ -128,7 +139,7 @@ __global__ void __launch_bounds__(NG_THREADS) ngram_kernel(NgArgs a) {
 TI_API int ti_ngram_drafts(int* tokens, int* counts, int* starts, int* lengths_out, int* history, const int* lengths, const int* state_slots,
                            const int* new_tokens, const int* new_counts, const int* limits, int* status, int requests, int rows, int room,
                            int new_width, int max_drafts, int min_match, int max_match, cudaStream_t stream) {
-    TI_REQUIRE(requests >= 0 && requests <= 65535 && rows >= 0 && room >= 0 && new_width >= 0 && new_width <= NG_MAX_NEW, "ngram_drafts: bad sizes");
+    TI_REQUIRE(requests >= 0 && requests <= 65535 && rows >= 0 && room >= 0 && room <= (1 << 30) && new_width >= 0 && new_width <= NG_MAX_NEW, "ngram_drafts: bad sizes");
     TI_REQUIRE(max_drafts >= 0 && max_drafts < NG_THREADS, "ngram_drafts: at most %d drafts", NG_THREADS - 1);
     TI_REQUIRE(min_match >= 1 && max_match >= min_match && max_match <= NG_MAX_MATCH, "ngram_drafts: matches of 1 to %d tokens", NG_MAX_MATCH);
     if (requests == 0) return 0;
@@ -136,7 +147,7 @@ TI_API int ti_ngram_drafts(int* tokens, int* counts, int* starts, int* lengths_o
              requests, rows, room, new_width, max_drafts, min_match, max_match};
     int ctas = 1;
     while (ctas < NG_CTAS && ctas * NG_LEAST < room) ctas *= 2;
-    ti_launch_clusters(ngram_kernel, dim3(ctas, requests), ctas, NG_THREADS, 0, stream, a);
+    ti_launch_clusters(ngram_kernel, dim3(ctas, requests), ctas, NG_THREADS, 0, true, stream, a);
     TI_CHECK_LAUNCH("ngram_drafts");
     return 0;
 }

@@ -45,7 +45,7 @@ constexpr int VD_CANDIDATES = 2048;  // of a top-k row, in shared memory
 constexpr int VD_MAX_VOCAB = 1 << 19;        // so many weights of at most 2^44 fit 64 bits
 constexpr int VD_LIST = 256;         // of what the threshold keeps, for the draw behind a draft that failed
 constexpr int VD_CTAS = 8;           // blocks that share such a draw
-constexpr int VD_STAGES = 6;         // groups of four tokens on their way to a thread there
+constexpr int VD_STAGES = 3;         // groups of four tokens on their way to a thread there
 constexpr float LOG2E = 1.4426950408889634f;
 
 // A warp's part of a row: the largest scaled logit, the sum of the exponentials relative to it, the best draw.
@@ -315,11 +315,14 @@ __device__ __forceinline__ RowStats whole_row(const VdArgs& a, const Place& at, 
     return st;
 }
 
+struct Range { unsigned least, most; };                       // of keys
+
 struct RowShared {
     unsigned key[VD_CANDIDATES];
     int idx[VD_CANDIDATES];
     int line[VD_CANDIDATES];         // the lines that hold candidates
-    unsigned hist[256], sel[2], top[VD_WARPS];
+    unsigned hist[256], sel[2];
+    Range range[VD_WARPS];
     float red[33];
     Best best[VD_WARPS];
     unsigned long long total[VD_WARPS];
@@ -339,12 +342,13 @@ __device__ __noinline__ int places_for(unsigned mask, int* counter) {
     return __shfl_sync(~0u, base, 31) + upto - n;
 }
 
-// The largest of the block's keys, two a thread.
-__device__ __noinline__ unsigned largest_key(unsigned one, unsigned two, unsigned* top_sh) {
-    const unsigned own = __reduce_max_sync(~0u, max(one, two));
-    if ((threadIdx.x & 31) == 0) top_sh[threadIdx.x >> 5] = own;
+// The least and the largest of the block's keys, two a thread; least: of those that are not 0.
+__device__ __noinline__ Range key_range(unsigned one, unsigned two, Range* sh) {
+    const unsigned least = __reduce_min_sync(~0u, min(one - 1u, two - 1u)), most = __reduce_max_sync(~0u, max(one, two));
+    if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = Range{least, most};
     __syncthreads();
-    return __reduce_max_sync(~0u, top_sh[threadIdx.x & (VD_WARPS - 1)]);
+    const Range of = sh[threadIdx.x & (VD_WARPS - 1)];
+    return Range{__reduce_min_sync(~0u, of.least) + 1u, __reduce_max_sync(~0u, of.most)};
 }
 
 // Of up to 512 keys, two a thread (0 where a thread has none; pairs: not all of the second are), of which at least k reach lo and none
@@ -448,7 +452,6 @@ __global__ void __launch_bounds__(VD_THREADS, 4) rows_kernel(VdArgs a) {
     RowStats st{0.f, 0.f, 0u, -1, 0.f, -1, {0, 0}};
     unsigned long long sum = 0;                              // weights of at most 1 in steps of 2^-44
     Best b{0.f, -1};
-    unsigned top;
     asm volatile("cp.async.wait_all;" ::: "memory");
 
     __syncthreads();
@@ -460,8 +463,8 @@ __global__ void __launch_bounds__(VD_THREADS, 4) rows_kernel(VdArgs a) {
         one = fmaxf(one, largest[i]);
         if (i + VD_THREADS < n_lines) two = fmaxf(two, largest[i + VD_THREADS]);
     }
-    top = largest_key(order_key(one), order_key(two), sh.top);
-    const unsigned bound = topk <= 2 * VD_THREADS ? reached_by(order_key(one), order_key(two), true, order_key(-INFINITY), top, topk, topk / 8)
+    const Range offered = key_range(order_key(one), order_key(two), sh.range);
+    const unsigned bound = topk <= 2 * VD_THREADS ? reached_by(order_key(one), order_key(two), true, offered.least, offered.most, topk, topk / 8)
                                                   : lines_reached_by(sh, largest, n_lines, topk);
     const float reached = key_value(bound), low = below_quotient(reached, temp);
     constexpr int FOURS = 5;                                 // groups of four a thread looks at together
@@ -520,9 +523,9 @@ __global__ void __launch_bounds__(VD_THREADS, 4) rows_kernel(VdArgs a) {
     if (fits && n <= 2 * VD_THREADS) {
         // fewer than k: no finite logit of the row is missing, and all are kept
         const unsigned first = tid < n ? sh.key[tid] : 0u, second = tid + VD_THREADS < n ? sh.key[tid + VD_THREADS] : 0u;
-        top = largest_key(first, second, sh.top);
-        if (n >= topk) st.threshold = reached_by(first, second, n > VD_THREADS, score_key(reached / temp), top, topk, 0);
-        st.m = n > 0 ? key_value(top) : -INFINITY;
+        const Range found = key_range(first, second, sh.range);
+        if (n >= topk) st.threshold = n == topk ? found.least : reached_by(first, second, n > VD_THREADS, found.least, found.most, topk, 0);
+        st.m = n > 0 ? key_value(found.most) : -INFINITY;
     } else {
         // many candidates; or more than there is room for (a k in the thousands, thousands of equal logits): the row itself
         auto scaled = [&](int i) { return fits ? key_value(sh.key[i]) : at.x[i] / temp; };
@@ -574,11 +577,13 @@ __global__ void __launch_bounds__(VD_THREADS, 4) rows_kernel(VdArgs a) {
 // Decides the request by its rows; if a drawn draft failed, draws from what is left of p beyond q. JUDGED: a cluster of blocks a
 // request, which share that draw's rows out; otherwise a block. GREEDY: every request is, and the rows' parts are met here.
 template <bool JUDGED, bool GREEDY>
-__global__ void __launch_bounds__(VD_THREADS, 4) verify_kernel(VdArgs a) {
+__global__ void __launch_bounds__(VD_THREADS, JUDGED ? 4 : 1) verify_kernel(VdArgs a) {
     __shared__ RowStats row_sh[2 * VD_MAX_DRAFTS + 1];
     __shared__ Best best_sh[VD_WARPS], part_sh[VD_CTAS];
     __shared__ int held_sh;
+    __shared__ unsigned beat_sh;
     ti_grid_launch_dependents();
+    if (threadIdx.x == 0) beat_sh = 0u;
     ti_grid_wait();
     const int r = blockIdx.y, tid = threadIdx.x, D = a.max_drafts, rank = blockIdx.x;
     const int2 rows = rows_of(a, r);
@@ -659,56 +664,63 @@ __global__ void __launch_bounds__(VD_THREADS, 4) verify_kernel(VdArgs a) {
                 // Logits that no threshold and no infinity cuts: a share is 2^(v c - m log2 e - log2 z). Otherwise by p_of and q_of.
                 const bool plain = !st.threshold && !ds.threshold && !pw.odd && !(failed && qw.odd) && st.z > 0.f;
                 const float p2 = pw.m2 + log2f(st.z), q2 = failed ? qw.m2 + log2f(ds.z) : INFINITY;
-                // Only tokens whose share can still pass the best B of the warp run: share / E > B needs 1 - U < share / B. 1 - U is
+                // Only tokens whose share can still pass the best B of the block run: share / E > B needs 1 - U < share / B. 1 - U is
                 // (2^23 - 1 - word / 2^9) / 2^23 + 2^-24, exactly; the first summand is had from the word's bits.
-                float spare = INFINITY;                      // 1 / B
+                unsigned beaten = 0u;                        // B as a key, as this warp knows it
+                float spare = INFINITY;                      // 1 / B, with something to spare
 #pragma unroll 1
                 for (int k = 0; k < VD_STAGES; ++k) fetch((rank + k * VD_CTAS) * VD_THREADS + tid, k);
                 int stage = 0;
 #pragma unroll 1
                 for (int g = rank * VD_THREADS + tid; g - tid < groups; g += stride) {
                     asm volatile("cp.async.wait_group %0;" ::"n"(VD_STAGES - 1) : "memory");
+                    const float4 f = *reinterpret_cast<const float4*>(ring + ((stage * 2) * VD_THREADS + tid) * 4);
+                    float4 o = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+                    if (failed) o = *reinterpret_cast<const float4*>(ring + ((stage * 2 + 1) * VD_THREADS + tid) * 4);
+                    const float v[4] = {f.x, f.y, f.z, f.w}, q[4] = {o.x, o.y, o.z, o.w};
                     float p[4], ahead = 0.f;
-                    {
-                        const float4 f = *reinterpret_cast<const float4*>(ring + ((stage * 2) * VD_THREADS + tid) * 4);
-                        p[0] = f.x; p[1] = f.y; p[2] = f.z; p[3] = f.w;
-                        float4 o = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
-                        if (failed) o = *reinterpret_cast<const float4*>(ring + ((stage * 2 + 1) * VD_THREADS + tid) * 4);
-                        const float q[4] = {o.x, o.y, o.z, o.w};
-                        if (plain) {
 #pragma unroll
-                            for (int i = 0; i < 4; ++i) p[i] = ex2(fmaf(fmaxf(p[i], -INFINITY), pw.c, -p2)) - ex2(fmaf(fmaxf(q[i], -INFINITY), pw.c, -q2));
-                        } else {
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) p[i] = p_of(p[i]) - (failed ? q_of(q[i]) : 0.f);
-                        }
-                        if (g >= groups) p[0] = p[1] = p[2] = p[3] = 0.f;
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) ahead = fmaxf(ahead, p[i]);
+                    for (int i = 0; i < 4; ++i) {
+                        if (plain) p[i] = ex2(fmaf(fmaxf(v[i], -INFINITY), pw.c, -p2)) - ex2(fmaf(fmaxf(q[i], -INFINITY), pw.c, -q2));
+                        else p[i] = p_of(v[i]) - (failed ? q_of(q[i]) : 0.f);
+                        if (g >= groups) p[i] = 0.f;
+                        ahead = fmaxf(ahead, p[i]);
                     }
                     fetch(g + VD_STAGES * stride, stage);    // (what lay there is in registers)
                     stage = stage + 1 < VD_STAGES ? stage + 1 : 0;
-                    unsigned run = 0u;
-                    if (spare == INFINITY || !plain) {       // nothing to beat yet: all of them
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) run |= p[i] > 0.f ? 1u << i : 0u;
-                    } else if (ahead * spare > 5.9e-8f) {    // 1 - U is 2^-24 at least
-                        const uint4 w = philox4x32_10(make_uint4((unsigned)g, c1, stream, domain), key2);
-                        const unsigned words[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-                        for (int i = 0; i < 4; ++i)
-                            run |= 1.99999988f - __uint_as_float(0x3F800000u | words[i] >> 9) < fmaf(p[i], spare, -5.9604645e-8f) ? 1u << i : 0u;
+                    const unsigned now = *reinterpret_cast<volatile unsigned*>(&beat_sh);
+                    if (now != beaten) {
+                        beaten = now;
+                        spare = pw.spare() * (failed ? 1.f / key_value(now) : ex2((st.m - key_value(now)) * LOG2E) * st.z);
                     }
-                    if (__any_sync(~0u, run)) {
+                    if (!__any_sync(~0u, plain ? ahead * spare > 5.9e-8f : ahead > 0.f)) continue;         // 1 - U is 2^-24 at least
+                    const uint4 w = philox4x32_10(make_uint4((unsigned)g, c1, stream, domain), key2);
+                    const unsigned words[4] = {w.x, w.y, w.z, w.w};
+                    bool again;
+                    do {
+                        again = plain && spare == INFINITY;  // nothing to beat yet: the foremost of every thread, then all
+                        unsigned run = 0u;
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const bool may = again ? p[i] == ahead : !plain || 1.99999988f - __uint_as_float(0x3F800000u | words[i] >> 9) < fmaf(p[i], spare, -5.9604645e-8f);
+                            run |= may && p[i] > 0.f ? 1u << i : 0u;
+                        }
+                        if (!__any_sync(~0u, run)) break;
 #pragma unroll 1
                         for (; run; run &= run - 1u) {
                             const int i = __ffs(run) - 1;
-                            if (failed) race(i & 2 ? (i & 1 ? p[3] : p[2]) : (i & 1 ? p[1] : p[0]), 4 * g + i);
-                            else b = better(b, Best{x[4 * g + i] / temp - logf(exponential_of(4 * g + i, c1, stream, domain, key2)), 4 * g + i});
+                            const float e = -logf(philox_uniform(word_of(w, i)));
+                            const float share = i & 2 ? (i & 1 ? p[3] : p[2]) : (i & 1 ? p[1] : p[0]);
+                            const float own = i & 2 ? (i & 1 ? v[3] : v[2]) : (i & 1 ? v[1] : v[0]);
+                            b = better(b, Best{failed ? share / e : own / temp - logf(e), 4 * g + i});
                         }
                         const unsigned best = __reduce_max_sync(~0u, b.i < 0 ? 0u : order_key(b.v));
-                        if (best) spare = pw.spare() * (failed ? 1.f / key_value(best) : ex2((st.m - key_value(best)) * LOG2E) * st.z);
-                    }
+                        if (best > beaten) {
+                            if ((tid & 31) == 0) atomicMax(&beat_sh, best);
+                            beaten = best;
+                            spare = pw.spare() * (failed ? 1.f / key_value(best) : ex2((st.m - key_value(best)) * LOG2E) * st.z);
+                        }
+                    } while (again && spare != INFINITY);
                 }
                 asm volatile("cp.async.wait_all;" ::: "memory");
                 b = block_best(b, best_sh);
@@ -774,7 +786,8 @@ TI_API int ti_verify_drafts(int* tokens, int* counts, float* accept, const float
     if (draft_logits) {
         constexpr int shared = VD_STAGES * 2 * VD_THREADS * 16;
         TI_REQUIRE((ti_allow_shared<verify_kernel<true, false>>(shared) == cudaSuccess), "verify_drafts: %d bytes of shared memory are not to be had", shared);
-        ti_launch_clusters(verify_kernel<true, false>, dim3(VD_CTAS, requests), VD_CTAS, VD_THREADS, shared, stream, a);
+        // started early its blocks lie where the kernel before ends first, several on an SM: 64 open requests x 7 drafts 144 us for 135
+        ti_launch_clusters(verify_kernel<true, false>, dim3(VD_CTAS, requests), VD_CTAS, VD_THREADS, shared, false, stream, a);
     }
     else ti_launch(temperature ? verify_kernel<false, false> : verify_kernel<false, true>, dim3(1, requests), VD_THREADS, 0, stream, a);
     TI_CHECK_LAUNCH("verify_drafts");

@@ -2402,6 +2402,7 @@ def _per_request(n: int, device, **tensors) -> None:
 
 
 _layouts = {}
+_NO_OPTIONS = (None,) * 6
 
 
 def _packed(device, *shapes):
@@ -2459,33 +2460,35 @@ def verify_drafts(logits: torch.Tensor, token_ids: torch.Tensor, cu_rows: torch.
         raise KernelError(f"verify_drafts: max_drafts must be 0 to {MAX_DRAFTS}, got {d}")
     if token_ids.device != device or cu_rows.device != device:
         raise KernelError("verify_drafts: all tensors lie on one device")
-    options = (temperature, topk, greedy, seed, stream_id, step)
-    given = sum(t is not None for t in options)
-    if given not in (0, 6):
-        raise KernelError("verify_drafts: the sampling options go together: temperature, topk, greedy, seed, stream_id, step")
+    sampled = temperature is not None
     stride_s = stride_d = 0
-    if given:
+    if not sampled:
+        options = _NO_OPTIONS
+        if not (topk is greedy is seed is stream_id is step is draft_logits is None):
+            raise KernelError("verify_drafts: the sampling options go together: temperature, topk, greedy, seed, stream_id, step; without "
+                              "them every request is greedy and draft_logits have no use")
+    else:
+        if topk is None or greedy is None or seed is None or stream_id is None or step is None:
+            raise KernelError("verify_drafts: the sampling options go together: temperature, topk, greedy, seed, stream_id, step")
         _per_request(s, device, temperature=(temperature, torch.float32), topk=(topk, torch.int32), greedy=(greedy, torch.int32),
                      seed=(seed, torch.int64), stream_id=(stream_id, torch.int32), step=(step, torch.int32))
-    if draft_logits is not None:
-        if not given:
-            raise KernelError("verify_drafts: without sampling options every request is greedy and draft_logits have no use")
-        if draft_logits.dtype != torch.float32 or draft_logits.device != device:
-            raise KernelError(f"draft_logits must be float32 on {device}, got {draft_logits.dtype} on {draft_logits.device}")
-        if tuple(draft_logits.shape) != (s, d, vocab) or (draft_logits.numel() and vocab > 1 and draft_logits.stride(2) != 1):
-            raise KernelError(f"draft_logits must be [{s}, {d}, {vocab}] with neighbouring tokens side by side, got "
-                              f"{tuple(draft_logits.shape)} with strides {draft_logits.stride()}")
-        stride_s, stride_d = draft_logits.stride(0), draft_logits.stride(1)
-        if d == 0:
-            draft_logits = None
+        options = (temperature.data_ptr(), topk.data_ptr(), greedy.data_ptr(), seed.data_ptr(), stream_id.data_ptr(), step.data_ptr())
+        if draft_logits is not None:
+            if draft_logits.dtype != torch.float32 or draft_logits.device != device:
+                raise KernelError(f"draft_logits must be float32 on {device}, got {draft_logits.dtype} on {draft_logits.device}")
+            if draft_logits.shape != (s, d, vocab) or (vocab > 1 and draft_logits.numel() and draft_logits.stride(2) != 1):
+                raise KernelError(f"draft_logits must be [{s}, {d}, {vocab}] with neighbouring tokens side by side, got "
+                                  f"{tuple(draft_logits.shape)} with strides {draft_logits.stride()}")
+            stride_s, stride_d = draft_logits.stride(0), draft_logits.stride(1)
+            if d == 0:
+                draft_logits = None
     _on_current(device)
     tokens, counts, accept = _packed(device, (s, d + 1), (s,), (s, d))
     accept = accept.view(torch.float32)
     # scratch of the call's own: calls on several streams, or in several captured graphs, do not meet in it
-    scratch = torch.empty(_verify_scratch_words(s, d, vocab, given > 0, draft_logits is not None), dtype=torch.int32, device=device)
+    scratch = torch.empty(_verify_scratch_words(s, d, vocab, sampled, draft_logits is not None), dtype=torch.int32, device=device)
     _run("drafts", "ti_verify_drafts", tokens.data_ptr(), counts.data_ptr(), accept.data_ptr(), logits.data_ptr(),
-         token_ids.data_ptr(), cu_rows.data_ptr(), n, vocab, s, d, *[_ptr(t) for t in options], _ptr(draft_logits), stride_s, stride_d,
-         scratch.data_ptr(), _stream())
+         token_ids.data_ptr(), cu_rows.data_ptr(), n, vocab, s, d, *options, _ptr(draft_logits), stride_s, stride_d, scratch.data_ptr(), _stream())
     return VerifiedDrafts(tokens, counts, accept)
 
 
@@ -2524,6 +2527,8 @@ def ngram_drafts(history: torch.Tensor, lengths: torch.Tensor, *, max_drafts: in
         raise KernelError(f"ngram_drafts: max_drafts must be 0 to {MAX_DRAFTS}, got {d}")
     if not 1 <= min_match <= max_match <= 32:
         raise KernelError(f"ngram_drafts: 1 <= min_match <= max_match <= 32, got {min_match} and {max_match}")
+    if history.shape[1] > 1 << 30:
+        raise KernelError("ngram_drafts: texts of at most 2^30 tokens")
     if state_slots is None and history.shape[0] < s:
         raise KernelError(f"ngram_drafts: {s} requests, but the history has {history.shape[0]} rows")
     if (tokens is None) != (counts is None):
