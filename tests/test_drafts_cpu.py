@@ -58,8 +58,7 @@ def ops(monkeypatch):
 
     calls = []
     monkeypatch.setattr(ops, "_check", check)
-    monkeypatch.setattr(ops, "_on_current", lambda device: None)
-    monkeypatch.setattr(ops, "_stream", lambda: 0)
+    monkeypatch.setattr(ops, "_stream_of", lambda device: 0)
     monkeypatch.setattr(ops, "_verify_scratch_words", lambda *a: 16)
     monkeypatch.setattr(ops, "_run", lambda lib, name, *args: calls.append((name, args)))
     ops_calls = ops

@@ -27,10 +27,12 @@ struct SaArgs {
 };
 
 // What request s brings: its count within the limits; none without a row of the tables or with a start that is no position.
+__device__ __forceinline__ bool is_there(const SaArgs& a, int slot, int start) {
+    return slot >= 0 && slot < a.table_rows && start >= 0 && start <= 0x7FFFFFFF - a.max_count;
+}
 __device__ __forceinline__ int brings(const SaArgs& a, int s, bool* cut) {
     const int slot = a.state_slots ? a.state_slots[s] : s, start = a.starts[s], count = a.counts[s];
-    const bool there = slot >= 0 && slot < a.table_rows && start >= 0 && start <= 0x7FFFFFFF - a.max_count;
-    const int n = there ? min(max(count, 0), a.max_count) : 0;
+    const int n = is_there(a, slot, start) ? min(max(count, 0), a.max_count) : 0;
     *cut = n != max(count, 0);
     return n;
 }
@@ -40,10 +42,17 @@ __global__ void __launch_bounds__(SA_THREADS) step_arrays_kernel(SaArgs a) {
     ti_grid_launch_dependents();
     ti_grid_wait();
     const int s = blockIdx.y, tid = threadIdx.x, parts = gridDim.x, part = blockIdx.x;
+    const bool pad = s == a.requests;
+    const int slot = pad ? 0 : (a.state_slots ? a.state_slots[s] : s), given = pad ? 0 : a.starts[s];
+    const bool there = pad || is_there(a, slot, given);
+    const int start = there ? given : 0;
+    bool cut = false;
+    const int wanted = pad ? a.rows : brings(a, s, &cut);
     // the counts before this request; a sum that passes the rows stays there
     int before = 0;
-    bool cut;
-    for (int i = tid; i < s; i += SA_THREADS) before = min(before + brings(a, i, &cut), a.rows);
+    bool other;
+#pragma unroll 4
+    for (int i = tid; i < s; i += SA_THREADS) before = min(before + brings(a, i, &other), a.rows);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) before = min(before + __shfl_xor_sync(~0u, before, o), a.rows);
     if ((tid & 31) == 0) sums[tid >> 5] = before;
@@ -51,14 +60,8 @@ __global__ void __launch_bounds__(SA_THREADS) step_arrays_kernel(SaArgs a) {
     before = 0;
 #pragma unroll
     for (int w = 0; w < SA_THREADS / 32; ++w) before = min(before + sums[w], a.rows);
-
-    const bool pad = s == a.requests;
-    cut = false;
-    int n = pad ? a.rows - before : brings(a, s, &cut);
-    if (!pad && n > a.rows - before) { n = a.rows - before; cut = true; }
-    const int slot = pad ? 0 : (a.state_slots ? a.state_slots[s] : s);
-    const bool there = pad || (slot >= 0 && slot < a.table_rows && a.starts[s] >= 0 && a.starts[s] <= 0x7FFFFFFF - a.max_count);
-    const int start = pad || !there ? 0 : a.starts[s];
+    const int n = min(wanted, a.rows - before);
+    if (!pad && n < wanted) cut = true;
     const int context = pad ? 1 : start + n;
     if (part == 0) {
         if (tid == 0) {
@@ -79,8 +82,8 @@ __global__ void __launch_bounds__(SA_THREADS) step_arrays_kernel(SaArgs a) {
     for (int g = 0; g < a.groups; ++g) {
         const int* table = a.tables + ((size_t)g * a.table_rows + slot) * a.width;
         int* to = a.block_tables + ((size_t)g * (a.requests + 1) + s) * a.width;
-        for (int i = part * SA_THREADS + tid; i < a.width; i += parts * SA_THREADS)
-            to[i] = pad ? (i == 0 ? a.pad_page : -1) : (i < held ? table[i] : -1);
+#pragma unroll 8
+        for (int i = part * SA_THREADS + tid; i < a.width; i += parts * SA_THREADS) to[i] = i < held ? (pad ? a.pad_page : table[i]) : -1;
     }
     // the tokens
     for (int i = part * SA_THREADS + tid; i < n; i += parts * SA_THREADS) {

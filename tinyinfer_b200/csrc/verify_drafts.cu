@@ -253,7 +253,7 @@ __global__ void __launch_bounds__(VD_THREADS, DRAWS ? 4 : 5) parts_kernel(VdArgs
         // The largest of s + G, G = -log E, E = -log U. A token can pass a score B only if E < exp(s - B); E is 1 - U at least, and 1 - U
         // is exact: one comparison settles all but a few tokens once some B is known.
         const uint2 key2 = seed_of(a, r);
-        const unsigned c1 = (unsigned)(a.step[r] + at.j), stream = (unsigned)a.stream_id[r];
+        const unsigned c1 = (unsigned)a.step[r] + (unsigned)at.j, stream = (unsigned)a.stream_id[r];
         float spare = 0.f;                                   // exp(m - B)
 #pragma unroll 1
         for (int half = 0; half < 2; ++half) {               // the threads' largest logits for a first B, then all
@@ -517,7 +517,7 @@ __global__ void __launch_bounds__(VD_THREADS, 4) rows_kernel(VdArgs a) {
         fits = sh.count <= VD_CANDIDATES;
     }
     const uint2 key2 = at.draws ? seed_of(a, r) : make_uint2(0u, 0u);
-    const unsigned c1 = at.draws ? (unsigned)(a.step[r] + at.j) : 0u, stream = at.draws ? (unsigned)a.stream_id[r] : 0u;
+    const unsigned c1 = at.draws ? (unsigned)a.step[r] + (unsigned)at.j : 0u, stream = at.draws ? (unsigned)a.stream_id[r] : 0u;
     Kept* kept = lists ? a.kept + ((size_t)r * D + at.j) * VD_LIST : nullptr;
     const int n = fits ? sh.count : a.vocab;
     if (fits && n <= 2 * VD_THREADS) {

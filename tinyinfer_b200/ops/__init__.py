@@ -2385,16 +2385,16 @@ class StepArrays(NamedTuple):
     block_tables: torch.Tensor            # int32 [groups, S + 1, width]
 
 
-def _on_current(device) -> None:
+def _stream_of(device) -> int:
+    """The current stream, of the device that the tensors lie on; kernels are launched on the current one."""
     if device.index != torch.cuda.current_device():
         raise KernelError(f"the tensors lie on {device}, the current device is cuda:{torch.cuda.current_device()}")
+    return _raw_stream(device.index) if _raw_stream is not None else _stream()
 
 
-def _per_request(n: int, device, **tensors) -> None:
-    """Checks tensors of one entry a request on one device: ``name=(tensor, dtype)``."""
-    for name, (t, dtype) in tensors.items():
-        if isinstance(t, torch.Tensor) and t.dtype is dtype and t.shape == (n,) and t.device == device and t.is_contiguous():
-            continue
+def _per_request(t: torch.Tensor, name: str, dtype, n: int, device) -> None:
+    """Checks a tensor of one entry a request."""
+    if not (isinstance(t, torch.Tensor) and t.dtype is dtype and t.device == device and t.shape == (n,) and t.is_contiguous()):
         _check(t, name, dtype, 1)
         if t.shape[0] != n:
             raise KernelError(f"{name} must have one entry per request: {n}, got {t.shape[0]}")
@@ -2403,11 +2403,13 @@ def _per_request(n: int, device, **tensors) -> None:
 
 _layouts = {}
 _NO_OPTIONS = (None,) * 6
+_SCRATCH_BEHIND = 1 << 18     # words of scratch (1 MB) that may lie behind a call's outputs
 
 
-def _packed(device, *shapes):
-    """Uninitialised int32 tensors of these shapes in one allocation, each on a 16-byte boundary. (An allocation of its own for each
-    takes the host two to four times as long, which is what the small kernels behind it wait for.)"""
+def _packed(device, *shapes, scratch: int = 0):
+    """Uninitialised int32 tensors of these shapes in one allocation, each on a 16-byte boundary, then the address of ``scratch`` words
+    behind them. (An allocation of its own for each takes the host two to four times as long, which is what the small kernels behind it
+    wait for.) The scratch is the call's own: calls on several streams, or in several captured graphs, do not meet in it."""
     layout = _layouts.get(shapes)
     if layout is None:
         views, at = [], 0
@@ -2421,8 +2423,9 @@ def _packed(device, *shapes):
         if len(_layouts) >= 4096:
             _layouts.clear()
         layout = _layouts[shapes] = (views, at)
-    buf = torch.empty(layout[1], dtype=torch.int32, device=device)
-    return [buf.as_strided(*view) for view in layout[0]]
+    views, words = layout
+    buf = torch.empty(words + scratch, dtype=torch.int32, device=device)
+    return [buf.as_strided(*view) for view in views] + [buf.data_ptr() + 4 * words]
 
 
 def verify_drafts(logits: torch.Tensor, token_ids: torch.Tensor, cu_rows: torch.Tensor, *, max_drafts: int,
@@ -2470,8 +2473,12 @@ def verify_drafts(logits: torch.Tensor, token_ids: torch.Tensor, cu_rows: torch.
     else:
         if topk is None or greedy is None or seed is None or stream_id is None or step is None:
             raise KernelError("verify_drafts: the sampling options go together: temperature, topk, greedy, seed, stream_id, step")
-        _per_request(s, device, temperature=(temperature, torch.float32), topk=(topk, torch.int32), greedy=(greedy, torch.int32),
-                     seed=(seed, torch.int64), stream_id=(stream_id, torch.int32), step=(step, torch.int32))
+        _per_request(temperature, "temperature", torch.float32, s, device)
+        _per_request(topk, "topk", torch.int32, s, device)
+        _per_request(greedy, "greedy", torch.int32, s, device)
+        _per_request(seed, "seed", torch.int64, s, device)
+        _per_request(stream_id, "stream_id", torch.int32, s, device)
+        _per_request(step, "step", torch.int32, s, device)
         options = (temperature.data_ptr(), topk.data_ptr(), greedy.data_ptr(), seed.data_ptr(), stream_id.data_ptr(), step.data_ptr())
         if draft_logits is not None:
             if draft_logits.dtype != torch.float32 or draft_logits.device != device:
@@ -2482,13 +2489,13 @@ def verify_drafts(logits: torch.Tensor, token_ids: torch.Tensor, cu_rows: torch.
             stride_s, stride_d = draft_logits.stride(0), draft_logits.stride(1)
             if d == 0:
                 draft_logits = None
-    _on_current(device)
-    tokens, counts, accept = _packed(device, (s, d + 1), (s,), (s, d))
+    stream = _stream_of(device)
+    words = _verify_scratch_words(s, d, vocab, sampled, draft_logits is not None)
+    large = torch.empty(words, dtype=torch.int32, device=device) if words > _SCRATCH_BEHIND else None    # outputs do not keep it alive
+    tokens, counts, accept, scratch = _packed(device, (s, d + 1), (s,), (s, d), scratch=0 if large is not None else words)
     accept = accept.view(torch.float32)
-    # scratch of the call's own: calls on several streams, or in several captured graphs, do not meet in it
-    scratch = torch.empty(_verify_scratch_words(s, d, vocab, sampled, draft_logits is not None), dtype=torch.int32, device=device)
     _run("drafts", "ti_verify_drafts", tokens.data_ptr(), counts.data_ptr(), accept.data_ptr(), logits.data_ptr(),
-         token_ids.data_ptr(), cu_rows.data_ptr(), n, vocab, s, d, *options, _ptr(draft_logits), stride_s, stride_d, scratch.data_ptr(), _stream())
+         token_ids.data_ptr(), cu_rows.data_ptr(), n, vocab, s, d, *options, _ptr(draft_logits), stride_s, stride_d, scratch if large is None else large.data_ptr(), stream)
     return VerifiedDrafts(tokens, counts, accept)
 
 
@@ -2537,16 +2544,18 @@ def ngram_drafts(history: torch.Tensor, lengths: torch.Tensor, *, max_drafts: in
         _check(tokens, "tokens", torch.int32, 2)
         if tokens.shape[0] != s or tokens.shape[1] > 512 or tokens.device != device:
             raise KernelError(f"ngram_drafts: tokens must be [{s}, at most 512] on {device}, got {tuple(tokens.shape)} on {tokens.device}")
-    for name, t in (("counts", counts), ("state_slots", state_slots), ("limits", limits)):
-        if t is not None:
-            _per_request(s, device, **{name: (t, torch.int32)})
+        _per_request(counts, "counts", torch.int32, s, device)
+    if state_slots is not None:
+        _per_request(state_slots, "state_slots", torch.int32, s, device)
+    if limits is not None:
+        _per_request(limits, "limits", torch.int32, s, device)
     if status is not None:
         _check(status, "status", torch.int32, 1)
-    _on_current(device)
-    out = NgramDrafts(*_packed(device, (s, d + 1), (s,), (s,), (s,)))
+    stream = _stream_of(device)
+    out = NgramDrafts(*_packed(device, (s, d + 1), (s,), (s,), (s,))[:4])
     _run("drafts", "ti_ngram_drafts", out.tokens.data_ptr(), out.counts.data_ptr(), out.starts.data_ptr(), out.lengths.data_ptr(),
          history.data_ptr(), lengths.data_ptr(), _ptr(state_slots), _ptr(tokens), _ptr(counts), _ptr(limits), _ptr(status), s,
-         history.shape[0], history.shape[1], tokens.shape[1] if tokens is not None else 0, d, int(min_match), int(max_match), _stream())
+         history.shape[0], history.shape[1], tokens.shape[1] if tokens is not None else 0, d, int(min_match), int(max_match), stream)
     return out
 
 
@@ -2569,9 +2578,9 @@ def step_arrays(starts: torch.Tensor, counts: torch.Tensor, block_tables: torch.
     rows, max_count, page_size, pad_page = int(rows), int(max_count), int(page_size), int(pad_page)
     _check(starts, "starts", torch.int32, 1)
     s, device = starts.shape[0], starts.device
-    _per_request(s, device, counts=(counts, torch.int32))
+    _per_request(counts, "counts", torch.int32, s, device)
     if state_slots is not None:
-        _per_request(s, device, state_slots=(state_slots, torch.int32))
+        _per_request(state_slots, "state_slots", torch.int32, s, device)
     if block_tables.dim() == 2:
         block_tables = block_tables.unsqueeze(0)
     _check(block_tables, "block_tables", torch.int32, 3)
@@ -2590,16 +2599,15 @@ def step_arrays(starts: torch.Tensor, counts: torch.Tensor, block_tables: torch.
                               f"{tokens.device}")
     if status is not None:
         _check(status, "status", torch.int32, 1)
-    _on_current(device)
+    stream = _stream_of(device)
     tiles = s * -(-max_count // STEP_TILE)
-    pos, seq, slots, cu, q_starts, ends, tile, table, *ids = _packed(
-        device, (rows,), (rows,), (groups, rows), (s + 2,), (s + 1,), (s + 1,), (tiles, 4), (groups, s + 1, width),
-        *([(rows,)] if tokens is not None else []))
-    flat = ids[0] if ids else None
+    shapes = ((rows,), (rows,), (groups, rows), (s + 2,), (s + 1,), (s + 1,), (tiles, 4), (groups, s + 1, width))
+    pos, seq, slots, cu, q_starts, ends, tile, table, flat, *_ = _packed(device, *shapes, (rows,)) if tokens is not None else [
+        *_packed(device, *shapes)[:8], None]
     _run("drafts", "ti_step_arrays", _ptr(flat), pos.data_ptr(), seq.data_ptr(), slots.data_ptr(), cu.data_ptr(), q_starts.data_ptr(),
          ends.data_ptr(), tile.data_ptr(), table.data_ptr(), starts.data_ptr(), counts.data_ptr(), _ptr(state_slots),
          block_tables.data_ptr(), _ptr(tokens), _ptr(status), s, groups, table_rows, width, tokens.shape[1] if tokens is not None else 0,
-         rows, max_count, page_size, pad_page, _stream())
+         rows, max_count, page_size, pad_page, stream)
     return StepArrays(flat, pos, seq, slots, cu, q_starts, ends, tile, table)
 
 
