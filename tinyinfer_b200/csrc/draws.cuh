@@ -29,9 +29,9 @@ __device__ __forceinline__ unsigned order_key(float v) {           // larger flo
     return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
 }
 
-// Launches `kernel` on clusters of `ctas` blocks along x; early: as ti_launch does, otherwise as ti_launch_alone.
+// Launches `kernel` on clusters of `ctas` blocks along x, otherwise as ti_launch does.
 template <typename... KArgs, typename... Args>
-cudaError_t ti_launch_clusters(void (*kernel)(KArgs...), dim3 grid, int ctas, dim3 block, size_t smem, bool early, cudaStream_t stream, Args... args) {
+cudaError_t ti_launch_clusters(void (*kernel)(KArgs...), dim3 grid, int ctas, dim3 block, size_t smem, cudaStream_t stream, Args... args) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = grid;
     cfg.blockDim = block;
@@ -44,8 +44,21 @@ cudaError_t ti_launch_clusters(void (*kernel)(KArgs...), dim3 grid, int ctas, di
     attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = early && ti_pdl_enabled() ? 2 : 1;
+    cfg.numAttrs = ti_pdl_enabled() ? 2 : 1;
     return cudaLaunchKernelEx(&cfg, kernel, KArgs(args)...);
+}
+
+// Lets KERNEL run on clusters of more than 8 blocks on the current device (the record as in ti_allow_shared).
+template <auto KERNEL>
+cudaError_t ti_allow_wide_clusters() {
+    constexpr int DEVICES = 64;
+    static bool allowed[DEVICES] = {};
+    int dev = -1;
+    const cudaError_t got = cudaGetDevice(&dev);
+    if (got != cudaSuccess || (dev < DEVICES && allowed[dev])) return got;
+    const cudaError_t e = cudaFuncSetAttribute(KERNEL, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    if (e == cudaSuccess && dev < DEVICES) allowed[dev] = true;
+    return e;
 }
 
 struct Best { float v; int i; };

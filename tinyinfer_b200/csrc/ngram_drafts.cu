@@ -147,7 +147,7 @@ TI_API int ti_ngram_drafts(int* tokens, int* counts, int* starts, int* lengths_o
              requests, rows, room, new_width, max_drafts, min_match, max_match};
     int ctas = 1;
     while (ctas < NG_CTAS && ctas * NG_LEAST < room) ctas *= 2;
-    ti_launch_clusters(ngram_kernel, dim3(ctas, requests), ctas, NG_THREADS, 0, true, stream, a);
+    ti_launch_clusters(ngram_kernel, dim3(ctas, requests), ctas, NG_THREADS, 0, stream, a);
     TI_CHECK_LAUNCH("ngram_drafts");
     return 0;
 }

@@ -43,8 +43,8 @@ constexpr int VD_TILE = VD_THREADS * VD_GROUPS * 4;
 constexpr int VD_LINE = 32;          // neighbouring logits that a top-k row's largest are taken of
 constexpr int VD_CANDIDATES = 2048;  // of a top-k row, in shared memory
 constexpr int VD_MAX_VOCAB = 1 << 19;        // so many weights of at most 2^44 fit 64 bits
-constexpr int VD_LIST = 256;         // of what the threshold keeps, for the draw behind a draft that failed
-constexpr int VD_CTAS = 8;           // blocks that share such a draw
+constexpr int VD_LIST = 1024;        // of what the threshold keeps, for the draw behind a draft that failed
+constexpr int VD_CTAS = 8, VD_MOST_CTAS = 16;         // blocks that share such a draw
 constexpr int VD_STAGES = 3;         // groups of four tokens on their way to a thread there
 constexpr float LOG2E = 1.4426950408889634f;
 
@@ -67,11 +67,11 @@ struct VdArgs {
     long long draft_request, draft_place;
     float* parts;                    // [requests, places, tiles, VD_THREADS]: lines' largest logits, or warps' Parts
     RowStats* stats;                 // [requests, places], where not all are greedy
-    Kept* kept;                      // [requests, max_drafts, VD_LIST]
+    Kept* kept;                      // [requests, max_drafts, list]
     int* tokens;                     // [requests, max_drafts + 1]
     int* counts;
     float* accept;                   // [requests, max_drafts]
-    int rows, vocab, requests, max_drafts, tiles;
+    int rows, vocab, requests, max_drafts, tiles, list;
     int places;                      // max_drafts + 1 rows of the target, then max_drafts of the draft model if there is one
 };
 
@@ -159,6 +159,21 @@ __device__ __forceinline__ void load_four(const float* x, int e, int vocab, int 
     } else {
 #pragma unroll
         for (int j = 0; j < 4; ++j) v[j] = e + j < vocab ? x[e + j] : NAN;
+    }
+}
+
+// f(logit, token) for all of a row, by the block; NaN for what lies behind it. Sixteen logits of a thread on their way at a time.
+template <typename F>
+__device__ __forceinline__ void each_of_row(const float* x, int vocab, int step, F f) {
+#pragma unroll 1
+    for (int first = 4 * (int)threadIdx.x; first < vocab; first += 16 * VD_THREADS) {
+        float v[4][4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) load_four(x, first + 4 * k * VD_THREADS, vocab, step, v[k]);
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) f(v[k][q], first + 4 * k * VD_THREADS + q);
     }
 }
 
@@ -466,7 +481,10 @@ __global__ void __launch_bounds__(VD_THREADS, 4) rows_kernel(VdArgs a) {
     const Range offered = key_range(order_key(one), order_key(two), sh.range);
     const unsigned bound = topk <= 2 * VD_THREADS ? reached_by(order_key(one), order_key(two), true, offered.least, offered.most, topk, topk / 8)
                                                   : lines_reached_by(sh, largest, n_lines, topk);
-    const float reached = key_value(bound), low = below_quotient(reached, temp);
+    // (What lies 110 below the largest, scaled, has no weight in float32 and no noise that makes up for it: the tokens that a mask of the
+    // type's lowest value leaves behind its own are not candidates, though the threshold may not drop them.)
+    const float most = key_value(offered.most), floor = fabsf(most / temp) < 1e30f ? most - 110.f * temp : -INFINITY;
+    const float low = fmaxf(below_quotient(key_value(bound), temp), floor);
     constexpr int FOURS = 5;                                 // groups of four a thread looks at together
 #pragma unroll 1
     for (int first = 0; first < n_lines; first += FOURS * 4 * VD_THREADS) {
@@ -518,8 +536,17 @@ __global__ void __launch_bounds__(VD_THREADS, 4) rows_kernel(VdArgs a) {
     }
     const uint2 key2 = at.draws ? seed_of(a, r) : make_uint2(0u, 0u);
     const unsigned c1 = at.draws ? (unsigned)a.step[r] + (unsigned)at.j : 0u, stream = at.draws ? (unsigned)a.stream_id[r] : 0u;
-    Kept* kept = lists ? a.kept + ((size_t)r * D + at.j) * VD_LIST : nullptr;
+    Kept* kept = lists ? a.kept + ((size_t)r * D + at.j) * a.list : nullptr;
     const int n = fits ? sh.count : a.vocab;
+    auto take = [&](float s, int token) {
+        if (score_key(s) < st.threshold) return;
+        sum += __float2ull_rn(scaled_weight(s, st.m) * 17592186044416.f);
+        if (at.draws) b = better(b, Best{s - logf(exponential_of(token, c1, stream, 0u, key2)), token});
+        if (lists && fits) {
+            const int to = atomicAdd(&sh.listed, 1);
+            if (to < a.list) kept[to] = Kept{s, token};
+        }
+    };
     if (fits && n <= 2 * VD_THREADS) {
         // fewer than k: no finite logit of the row is missing, and all are kept
         const unsigned first = tid < n ? sh.key[tid] : 0u, second = tid + VD_THREADS < n ? sh.key[tid + VD_THREADS] : 0u;
@@ -528,30 +555,25 @@ __global__ void __launch_bounds__(VD_THREADS, 4) rows_kernel(VdArgs a) {
         st.m = n > 0 ? key_value(found.most) : -INFINITY;
     } else {
         // many candidates; or more than there is room for (a k in the thousands, thousands of equal logits): the row itself
-        auto scaled = [&](int i) { return fits ? key_value(sh.key[i]) : at.x[i] / temp; };
-        if (n >= topk)
-            st.threshold = select_kth(topk, sh.hist, sh.sel, [&](auto count) {
-                for (int i = tid; i < n; i += VD_THREADS) {
-                    const float s = scaled(i);
-                    if (s == s) count(score_key(s));
-                }
-            });
+        auto each = [&](auto f) {                            // every candidate's scaled logit
+            if (fits) {
+                for (int i = tid; i < n; i += VD_THREADS) f(key_value(sh.key[i]), sh.idx[i]);
+            } else {
+                each_of_row(at.x, a.vocab, step, [&](float v, int i) { if (v >= low && v > -INFINITY) f(v / temp, i); });
+            }
+        };
+        if (n >= topk) st.threshold = select_kth(topk, sh.hist, sh.sel, [&](auto count) { each([&](float s, int) { count(score_key(s)); }); });
         float largest_scaled = -INFINITY;
-        for (int i = tid; i < n; i += VD_THREADS) largest_scaled = fmaxf(largest_scaled, scaled(i));
+        each([&](float s, int) { largest_scaled = fmaxf(largest_scaled, s); });
         st.m = block_max(largest_scaled, sh.red);
-        if (!fits && tid == 0) sh.listed = VD_LIST + 1;
-    }
-#pragma unroll 1
-    for (int i = tid; i < n; i += VD_THREADS) {
-        const float s = fits ? key_value(sh.key[i]) : at.x[i] / temp;
-        if (!(s > -INFINITY) || score_key(s) < st.threshold) continue;
-        const int token = fits ? sh.idx[i] : i;
-        sum += __float2ull_rn(scaled_weight(s, st.m) * 17592186044416.f);
-        if (at.draws) b = better(b, Best{s - logf(exponential_of(token, c1, stream, 0u, key2)), token});
-        if (lists && fits) {
-            const int to = atomicAdd(&sh.listed, 1);
-            if (to < VD_LIST) kept[to] = Kept{s, token};
+        if (!fits) {
+            each([&](float s, int token) { take(s, token); });
+            if (tid == 0) sh.listed = a.list + 1;
         }
+    }
+    if (fits) {
+#pragma unroll 1
+        for (int i = tid; i < n; i += VD_THREADS) take(key_value(sh.key[i]), sh.idx[i]);
     }
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
     b = warp_best(b);
@@ -570,7 +592,7 @@ __global__ void __launch_bounds__(VD_THREADS, 4) rows_kernel(VdArgs a) {
     st.drawn = b.i;
     const float s = at_draft / temp;
     if (s > -INFINITY && score_key(s) >= st.threshold) st.share = scaled_weight(s, st.m) / st.z;
-    if (lists && sh.listed <= VD_LIST) st.listed = sh.listed;
+    if (lists && sh.listed <= a.list) st.listed = sh.listed;
     a.stats[slot] = st;
 }
 
@@ -579,7 +601,7 @@ __global__ void __launch_bounds__(VD_THREADS, 4) rows_kernel(VdArgs a) {
 template <bool JUDGED, bool GREEDY>
 __global__ void __launch_bounds__(VD_THREADS, JUDGED ? 4 : 1) verify_kernel(VdArgs a) {
     __shared__ RowStats row_sh[2 * VD_MAX_DRAFTS + 1];
-    __shared__ Best best_sh[VD_WARPS], part_sh[VD_CTAS];
+    __shared__ Best best_sh[VD_WARPS], part_sh[VD_MOST_CTAS];
     __shared__ int held_sh;
     __shared__ unsigned beat_sh;
     ti_grid_launch_dependents();
@@ -647,13 +669,17 @@ __global__ void __launch_bounds__(VD_THREADS, JUDGED ? 4 : 1) verify_kernel(VdAr
             b.i = -1;
             if (failed && st.listed >= 0) {                  // the threshold keeps few: the first block alone
                 if (rank != 0) return;
-                const Kept* list = a.kept + ((size_t)r * D + held) * VD_LIST;
-                for (int i = tid; i < st.listed; i += VD_THREADS) race(scaled_weight(list[i].s, st.m) * pz - q_of(y[list[i].i]), list[i].i);
-                b = block_best(b, best_sh);
+                const Kept* list = a.kept + ((size_t)r * D + held) * a.list;
+                // (second: nothing of p lies beyond q, they differ by a rounding: p itself)
+#pragma unroll 1
+                for (float q_share = 1.f; q_share >= 0.f && b.i < 0; q_share -= 1.f) {
+                    for (int i = tid; i < st.listed; i += VD_THREADS) race(scaled_weight(list[i].s, st.m) * pz - q_share * q_of(y[list[i].i]), list[i].i);
+                    b = block_best(b, best_sh);
+                }
             } else {
                 cg::cluster_group cluster = cg::this_cluster();
                 extern __shared__ __align__(16) float ring[];                  // [stage][row][thread][4]: a thread's own
-                const int groups = (a.vocab + 3) / 4, stride = VD_CTAS * VD_THREADS, x_step = row_step(x), y_step = row_step(y);
+                const int groups = (a.vocab + 3) / 4, ctas = gridDim.x, stride = ctas * VD_THREADS, x_step = row_step(x), y_step = row_step(y);
                 auto fetch = [&](int g, int stage) {
                     if (g < groups) {
                         copy_four(ring + ((stage * 2) * VD_THREADS + tid) * 4, x, 4 * g, a.vocab, x_step);
@@ -669,7 +695,7 @@ __global__ void __launch_bounds__(VD_THREADS, JUDGED ? 4 : 1) verify_kernel(VdAr
                 unsigned beaten = 0u;                        // B as a key, as this warp knows it
                 float spare = INFINITY;                      // 1 / B, with something to spare
 #pragma unroll 1
-                for (int k = 0; k < VD_STAGES; ++k) fetch((rank + k * VD_CTAS) * VD_THREADS + tid, k);
+                for (int k = 0; k < VD_STAGES; ++k) fetch((rank + k * ctas) * VD_THREADS + tid, k);
                 int stage = 0;
 #pragma unroll 1
                 for (int g = rank * VD_THREADS + tid; g - tid < groups; g += stride) {
@@ -728,10 +754,10 @@ __global__ void __launch_bounds__(VD_THREADS, JUDGED ? 4 : 1) verify_kernel(VdAr
                 if (tid == 0) *cluster.map_shared_rank(&part_sh[rank], 0) = b;
                 cluster.sync();
                 if (rank != 0) return;
-                b = warp_best((tid & 31) < VD_CTAS ? part_sh[tid & 31] : Best{0.f, -1});
+                b = warp_best((tid & 31) < ctas ? part_sh[tid & 31] : Best{0.f, -1});
             }
-            if (b.i < 0 && failed) {                         // nothing of p lies beyond q (they differ by a rounding): p itself
-                for (int i = tid; i < a.vocab; i += VD_THREADS) race(p_of(x[i]), i);
+            if (b.i < 0 && failed) {                         // nothing of p lies beyond q, as above
+                each_of_row(x, a.vocab, row_step(x), [&](float v, int i) { race(p_of(v), i); });
                 b = block_best(b, best_sh);
             }
         }
@@ -743,14 +769,15 @@ __global__ void __launch_bounds__(VD_THREADS, JUDGED ? 4 : 1) verify_kernel(VdAr
     }
 }
 
-struct Scratch { long long parts, stats, kept, words; };      // offsets in words (32 bits)
+struct Scratch { long long parts, stats, kept, words; int list; };      // offsets in words (32 bits)
 Scratch scratch_of(int requests, int max_drafts, int vocab, bool sampled, bool draft_logits) {
     const long long places = draft_logits ? 2 * max_drafts + 1 : max_drafts + 1, tiles = (vocab + VD_TILE - 1) / VD_TILE;
     Scratch s;
     s.parts = 0;
     s.stats = s.parts + requests * places * tiles * VD_THREADS;
     s.kept = s.stats + (sampled ? requests * places * (long long)(sizeof(RowStats) / 4) : 0);
-    s.words = s.kept + (draft_logits ? (long long)requests * max_drafts * VD_LIST * (long long)(sizeof(Kept) / 4) : 0);
+    s.list = std::min(vocab, VD_LIST);
+    s.words = s.kept + (draft_logits ? (long long)requests * max_drafts * s.list * (long long)(sizeof(Kept) / 4) : 0);
     return s;
 }
 
@@ -774,7 +801,7 @@ TI_API int ti_verify_drafts(int* tokens, int* counts, float* accept, const float
     float* words = (float*)scratch;
     VdArgs a{logits, token_ids, cu_rows, temperature, topk, greedy, seed, stream_id, step, draft_logits, draft_request, draft_place,
              words + s.parts, (RowStats*)(words + s.stats), (Kept*)(words + s.kept), tokens, counts, accept, rows, vocab, requests, max_drafts,
-             (vocab + VD_TILE - 1) / VD_TILE, draft_logits ? 2 * max_drafts + 1 : max_drafts + 1};
+             (vocab + VD_TILE - 1) / VD_TILE, s.list, draft_logits ? 2 * max_drafts + 1 : max_drafts + 1};
     ti_launch(draft_logits || !temperature ? parts_kernel<false> : parts_kernel<true>, dim3(a.tiles, a.places, requests), VD_THREADS, 0, stream, a);
     TI_CHECK_LAUNCH("verify_drafts: parts");
     if (temperature) {
@@ -786,8 +813,11 @@ TI_API int ti_verify_drafts(int* tokens, int* counts, float* accept, const float
     if (draft_logits) {
         constexpr int shared = VD_STAGES * 2 * VD_THREADS * 16;
         TI_REQUIRE((ti_allow_shared<verify_kernel<true, false>>(shared) == cudaSuccess), "verify_drafts: %d bytes of shared memory are not to be had", shared);
-        // started early its blocks lie where the kernel before ends first, several on an SM: 64 open requests x 7 drafts 144 us for 135
-        ti_launch_clusters(verify_kernel<true, false>, dim3(VD_CTAS, requests), VD_CTAS, VD_THREADS, shared, false, stream, a);
+        // Sixteen blocks a request while all of them run at once, otherwise eight: 32 requests x 4 drafts, of which 8 are open, 45 us for 49;
+        // 64 open requests x 7 drafts 146 us for 135.
+        const bool wide = requests * VD_MOST_CTAS <= 148 * 4 && ti_allow_wide_clusters<verify_kernel<true, false>>() == cudaSuccess;
+        const int ctas = wide ? VD_MOST_CTAS : VD_CTAS;
+        ti_launch_clusters(verify_kernel<true, false>, dim3(ctas, requests), ctas, VD_THREADS, shared, stream, a);
     }
     else ti_launch(temperature ? verify_kernel<false, false> : verify_kernel<false, true>, dim3(1, requests), VD_THREADS, 0, stream, a);
     TI_CHECK_LAUNCH("verify_drafts");
