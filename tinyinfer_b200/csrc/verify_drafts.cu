@@ -123,6 +123,10 @@ struct Weights {
 // The same of a scaled logit at hand.
 __device__ __forceinline__ float scaled_weight(float s, float m) { return !(s > -INFINITY) ? 0.f : (s == m ? 1.f : ex2((s - m) * LOG2E)); }
 
+// Whether 1 - U < x for the uniform number U of a word of the stream. 1 - U is (2^23 - 1 - word / 2^9) / 2^23 + 2^-24, exactly; the first
+// summand is had from the word's bits by one subtraction.
+__device__ __forceinline__ bool may_pass(unsigned word, float x) { return 1.99999988f - __uint_as_float(0x3F800000u | word >> 9) < x - 5.9604645e-8f; }
+
 // s + G of a scaled logit s and its uniform number.
 __device__ __forceinline__ float noisy(float s, float u) { return s - logf(-logf(u)); }
 
@@ -183,6 +187,7 @@ __device__ __forceinline__ int token_of(int tile, int t, int k) { return tile * 
 // DRAWS: open rows draw here, too (drafts that nothing judges: every row's token is wanted).
 template <bool DRAWS>
 __global__ void __launch_bounds__(VD_THREADS, DRAWS ? 4 : 5) parts_kernel(VdArgs a) {
+    __shared__ float best_sh[VD_WARPS];
     ti_grid_launch_dependents();
     ti_grid_wait();
     const int tid = threadIdx.x, lane = tid & 31, r = blockIdx.z;
@@ -264,7 +269,7 @@ __global__ void __launch_bounds__(VD_THREADS, DRAWS ? 4 : 5) parts_kernel(VdArgs
     }
     z = warp_sum(z);
     Best b{-INFINITY, -1};
-    if (DRAWS && m > -INFINITY) {
+    if (DRAWS) {
         // The largest of s + G, G = -log E, E = -log U. A token can pass a score B only if E < exp(s - B); E is 1 - U at least, and 1 - U
         // is exact: one comparison settles all but a few tokens once some B is known.
         const uint2 key2 = seed_of(a, r);
@@ -279,11 +284,13 @@ __global__ void __launch_bounds__(VD_THREADS, DRAWS ? 4 : 5) parts_kernel(VdArgs
 #pragma unroll
                     for (int q = 0; q < 4; ++q) left = v[k][q] == most ? 1u << (4 * k + q) : left;
                 } else {
-                    const uint4 w = philox4x32_10(make_uint4((unsigned)token_of(blockIdx.x, tid, k) >> 2, c1, stream, 0u), key2);
+                    uint2 key = key2;                        // its ten bumps are made anew for every block: kept, they cost twenty registers
+                    asm volatile("" : "+r"(key.x), "+r"(key.y));
+                    const uint4 w = philox4x32_10(make_uint4((unsigned)token_of(blockIdx.x, tid, k) >> 2, c1, stream, 0u), key);
                     const unsigned words[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
                     for (int q = 0; q < 4; ++q)
-                        left |= (weight.odd ? v[k][q] > -INFINITY : 1.f - philox_uniform(words[q]) < v[k][q] * spare) ? 1u << (4 * k + q) : 0u;
+                        left |= (weight.odd ? v[k][q] > -INFINITY : may_pass(words[q], v[k][q] * spare)) ? 1u << (4 * k + q) : 0u;
                 }
             }
             if (half == 0 && !(most > (weight.odd ? -INFINITY : 0.f))) left = 0u;       // (a weight of nothing is beaten by the largest)
@@ -292,7 +299,12 @@ __global__ void __launch_bounds__(VD_THREADS, DRAWS ? 4 : 5) parts_kernel(VdArgs
                 const uint4 w = philox4x32_10(make_uint4((unsigned)i >> 2, c1, stream, 0u), key2);
                 b = better(b, Best{noisy(at.x[i] / temp, philox_uniform(word_of(w, i))), i});
             }
-            if (!weight.odd) spare = ex2((m - warp_max(b.v)) * LOG2E) * weight.spare();
+            if (half == 0) {                                 // the best that any warp of the block has found
+                const float own = warp_max(b.i < 0 ? -INFINITY : b.v);
+                if (lane == 0) best_sh[tid >> 5] = own;
+                __syncthreads();
+                spare = ex2((m - warp_max(best_sh[lane & (VD_WARPS - 1)])) * LOG2E) * weight.spare();
+            }
         }
         b = warp_best(b);
     }
@@ -690,8 +702,7 @@ __global__ void __launch_bounds__(VD_THREADS, JUDGED ? 4 : 1) verify_kernel(VdAr
                 // Logits that no threshold and no infinity cuts: a share is 2^(v c - m log2 e - log2 z). Otherwise by p_of and q_of.
                 const bool plain = !st.threshold && !ds.threshold && !pw.odd && !(failed && qw.odd) && st.z > 0.f;
                 const float p2 = pw.m2 + log2f(st.z), q2 = failed ? qw.m2 + log2f(ds.z) : INFINITY;
-                // Only tokens whose share can still pass the best B of the block run: share / E > B needs 1 - U < share / B. 1 - U is
-                // (2^23 - 1 - word / 2^9) / 2^23 + 2^-24, exactly; the first summand is had from the word's bits.
+                // Only tokens whose share can still pass the best B of the block run: share / E > B needs 1 - U < share / B.
                 unsigned beaten = 0u;                        // B as a key, as this warp knows it
                 float spare = INFINITY;                      // 1 / B, with something to spare
 #pragma unroll 1
@@ -728,7 +739,7 @@ __global__ void __launch_bounds__(VD_THREADS, JUDGED ? 4 : 1) verify_kernel(VdAr
                         unsigned run = 0u;
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
-                            const bool may = again ? p[i] == ahead : !plain || 1.99999988f - __uint_as_float(0x3F800000u | words[i] >> 9) < fmaf(p[i], spare, -5.9604645e-8f);
+                            const bool may = again ? p[i] == ahead : !plain || may_pass(words[i], p[i] * spare);
                             run |= may && p[i] > 0.f ? 1u << i : 0u;
                         }
                         if (!__any_sync(~0u, run)) break;
