@@ -8,6 +8,7 @@ few layers: the workload for per-kernel rooflines and for profiler captures.
     python benchmarks/kernel_microbench.py --kernel attention_prefill --tokens 2048
     python benchmarks/kernel_microbench.py --kernel rope_append --tokens 2048
     python benchmarks/kernel_microbench.py --kernel sample --batch 64 --topk 100
+    python benchmarks/kernel_microbench.py --kernel verify_drafts --batch 64 --drafts 4 --topk 100 --draft-logits
     python benchmarks/kernel_microbench.py --kernel decode_step --batch 8 --context 4096 --layers 4
     python benchmarks/kernel_microbench.py --kernel prefill_step --tokens 2048 --layers 4
 
@@ -64,9 +65,11 @@ def graph_time(fn, iters, use_graph=True):
 def main():
     ap = argparse.ArgumentParser(description=__doc__, formatter_class=argparse.RawDescriptionHelpFormatter)
     ap.add_argument("--kernel", required=True, choices=["gemm", "gated_gemm", "attention_decode", "attention_prefill",
-                                                       "rmsnorm", "rope_append", "sample", "decode_step", "prefill_step"])
+                                                       "rmsnorm", "rope_append", "sample", "decode_step", "prefill_step", "verify_drafts", "ngram_drafts", "step_arrays"])
     ap.add_argument("--topk", type=int, default=0, help="sample: top-k of every row (0: none; -1: every row greedy)")
     ap.add_argument("--vocab", type=int, default=151936)
+    ap.add_argument("--drafts", type=int, default=4, help="verify_drafts, ngram_drafts, step_arrays: drafts a request")
+    ap.add_argument("--draft-logits", action="store_true", help="verify_drafts: the drafts were drawn from a draft model's logits")
     ap.add_argument("--m", type=int, default=8)
     ap.add_argument("--n", type=int, default=4096)
     ap.add_argument("--k", type=int, default=4096)
@@ -131,6 +134,38 @@ def main():
         step = torch.zeros(n, dtype=torch.int32, device=dev)
         us = graph_time(lambda: ops.sample(logits, temp, topk, greedy, seed, stream_id, step), a.iters, not a.no_graph)
         out.update(rows=n, vocab=v, topk=a.topk, us=us, gbs=n * v * 4 / us / 1e3, tflops=0.0)
+    elif a.kernel in ("verify_drafts", "ngram_drafts", "step_arrays"):
+        n, d, v = a.batch, a.drafts, a.vocab
+
+        def ints(*values):
+            return torch.tensor(values, dtype=torch.int32, device=dev)
+
+        if a.kernel == "verify_drafts":
+            rows = n * (d + 1)
+            logits = torch.randn(rows, v, device=dev) * 3.0
+            draft_logits = (logits.view(n, d + 1, v)[:, :d] + 0.8 * torch.randn(n, d, v, device=dev)).contiguous() if a.draft_logits else None
+            fed = torch.randint(0, v, (n, d + 1), device=dev, dtype=torch.int32)
+            fed[:, 1:] = (logits if draft_logits is None else draft_logits).view(n, -1, v)[:, :d].argmax(2)
+            options = {} if a.topk < 0 else dict(
+                temperature=torch.full((n,), 0.7, device=dev), topk=ints(*[a.topk] * n), greedy=ints(*[0] * n), stream_id=ints(*range(n)),
+                seed=torch.arange(n, dtype=torch.int64, device=dev), step=ints(*[0] * n), draft_logits=draft_logits)
+            fed, cu = fed.flatten(), torch.arange(0, rows + 1, d + 1, dtype=torch.int32, device=dev)
+            us = graph_time(lambda: ops.verify_drafts(logits, fed, cu, max_drafts=d, **options), a.iters, not a.no_graph)
+            byts = 4.0 * v * (rows + (n * d if draft_logits is not None else 0))
+        elif a.kernel == "ngram_drafts":
+            history = torch.randint(0, 4000, (n, a.context + d + 1), device=dev, dtype=torch.int32)
+            lengths, found = ints(*[a.context] * n), torch.randint(0, 4000, (n, d + 1), device=dev, dtype=torch.int32)
+            counts = ints(*[1 + i % (d + 1) for i in range(n)])
+            us = graph_time(lambda: ops.ngram_drafts(history, lengths, max_drafts=d, tokens=found, counts=counts), a.iters, not a.no_graph)
+            byts = 4.0 * n * a.context
+        else:
+            width = -(-(a.context + d + 1) // a.page_size)
+            tables = torch.arange(n * width, dtype=torch.int32, device=dev).view(1, n, width)
+            starts, counts, fed = ints(*[a.context] * n), ints(*[d + 1] * n), torch.zeros(n, d + 1, dtype=torch.int32, device=dev)
+            us = graph_time(lambda: ops.step_arrays(starts, counts, tables, rows=n * (d + 1), max_count=d + 1, page_size=a.page_size,
+                                                    tokens=fed), a.iters, not a.no_graph)
+            byts = 8.0 * n * width + 20.0 * n * (d + 1)
+        out.update(batch=n, drafts=d, vocab=v, topk=a.topk, context=a.context, us=us, gbs=byts / us / 1e3, tflops=0.0)
     elif a.kernel == "rope_append":
         hq, hkv, d, page, t = a.heads, a.kv_heads, a.head_dim, a.page_size, a.tokens
         qkv = torch.randn(t, (hq + 2 * hkv) * d, device=dev).bfloat16()
