@@ -200,6 +200,45 @@ def test_masks_and_values_that_are_no_numbers(ops, vocab):
         check(ops, logits, fed, counts, d, opts, q)
 
 
+@pytest.mark.parametrize("with_q", [False, True])
+def test_thresholds_in_the_thousands(ops, with_q):
+    """More tokens kept than a block has room for, by a large k or by equal logits: the row itself is gone over."""
+    vocab, ks = 50021, [1023, 1025, 1500, 2047, 2100, 3500, 9000, 50000]
+    counts = [3] * len(ks)
+    logits, fed = batch(counts, vocab, seed=9, hit=0.7)
+    opts = options(len(ks), 9, topk=ks, temperature=[0.8, 1.0] * 4)
+    check(ops, logits, fed, counts, 2, opts, near(logits, counts, 2, 9) if with_q else None)
+    x = logits.view(len(ks), 3, vocab)
+    x[0, 0, ::7] = 9.0                                   # 7,146 equal logits above all but a few
+    x[1, :, 100:2600] = 30.0                             # 2,500 above all
+    x[2] = 1.0                                           # all of them
+    x[3, 1, :] = NEG
+    x[3, 1, :3000] = torch.linspace(-1, 1, 3000, device=dev())           # fewer than k are left
+    opts = options(len(ks), 10, topk=[10, 100, 5, 4000, 40, 40, 40, 40], temperature=[0.8, 1.0] * 4)
+    check(ops, logits, fed, counts, 2, opts, near(logits.nan_to_num(0.0, 20.0, -20.0), counts, 2, 10) if with_q else None,
+          may_skip=0.3)
+
+
+def test_many_requests_and_the_largest_vocabulary(ops):
+    rng = np.random.RandomState(4)
+    counts = rng.randint(0, 4, 400).tolist()
+    logits, fed = batch(counts, 300, seed=13)
+    opts = options(400, 13, topk=rng.choice([0, 1, 20, 299], 400).tolist(), greedy=rng.choice([0, 0, 1], 400).tolist(),
+                   temperature=rng.choice([0.5, 1.0, 1.5], 400).tolist())
+    check(ops, logits, fed, counts, 3, opts)
+    check(ops, logits, fed, counts, 3, opts, near(logits, counts, 3, 13))
+    for vocab in (1 << 19, (1 << 19) + 1):
+        x = torch.randn(2, vocab, device=dev())
+        x[0, vocab - 1] = 12.0
+        one = options(1, 1, topk=[50])
+        if vocab > 1 << 19:
+            with pytest.raises(ops.KernelError, match="vocabulary"):
+                ops.verify_drafts(x, ints([0, vocab - 1]), ints([0, 2]), max_drafts=1, **one)
+            continue
+        for opts in (None, one, options(1, 2)):
+            check(ops, x, [0, vocab - 1], [2], 1, opts, may_skip=1)
+
+
 def test_temperatures(ops):
     counts = [3] * 6
     logits, fed = batch(counts, 3001, seed=8, hit=0.5)

@@ -2434,8 +2434,8 @@ def verify_drafts(logits: torch.Tensor, token_ids: torch.Tensor, cu_rows: torch.
                   stream_id: Optional[torch.Tensor] = None, step: Optional[torch.Tensor] = None,
                   draft_logits: Optional[torch.Tensor] = None) -> VerifiedDrafts:
     """Which drafted tokens hold, and the token behind them. Request r brought the tokens ``token_ids[cu_rows[r] : cu_rows[r + 1]]``
-    (int32 [N]; ``cu_rows`` int32 [S + 1]), one that is settled and up to ``max_drafts`` drafts, and ``logits`` float32 [N, V] has the
-    row behind each: row j judges draft j, the last row is for the token behind all of them. Rows past ``max_drafts + 1`` of a request
+    (int32 [N]; ``cu_rows`` int32 [S + 1]), one that is settled and up to ``max_drafts`` drafts, and ``logits`` float32 [N, V] (V up to
+    524,288) has the row behind each: row j judges draft j, the last row is for the token behind all of them. Rows past ``max_drafts + 1`` of a request
     and rows that no request claims are not looked at; a request without rows gets no token.
 
     The sampling options are those of ``sample``, one entry per request; ``step`` counts for the request's first row, row j draws at
