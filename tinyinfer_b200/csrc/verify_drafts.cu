@@ -411,12 +411,15 @@ __device__ __noinline__ unsigned lines_reached_by(RowShared& sh, const float* la
     return lo;
 }
 
+__device__ __forceinline__ void copy_16(float* to, const float* from) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(to)), "l"(from) : "memory");
+}
 // Copies four neighbouring logits (NaN behind the row's end) to shared memory, for the thread that asks.
 __device__ __forceinline__ void copy_four(float* to, const float* x, int e, int vocab, int step) {
     const uint32_t d = (uint32_t)__cvta_generic_to_shared(to);
     const float* from = x + e;
     if (step == 4 && e + 3 < vocab) {
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(d), "l"(from) : "memory");
+        copy_16(to, from);
     } else if (step == 2 && e + 3 < vocab) {
         asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(d), "l"(from) : "memory");
         asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(d + 8), "l"(from + 2) : "memory");
@@ -692,10 +695,16 @@ __global__ void __launch_bounds__(VD_THREADS, JUDGED ? 4 : 1) verify_kernel(VdAr
                 cg::cluster_group cluster = cg::this_cluster();
                 extern __shared__ __align__(16) float ring[];                  // [stage][row][thread][4]: a thread's own
                 const int groups = (a.vocab + 3) / 4, ctas = gridDim.x, stride = ctas * VD_THREADS, x_step = row_step(x), y_step = row_step(y);
-                auto fetch = [&](int g, int stage) {
-                    if (g < groups) {
-                        copy_four(ring + ((stage * 2) * VD_THREADS + tid) * 4, x, 4 * g, a.vocab, x_step);
-                        if (failed) copy_four(ring + ((stage * 2 + 1) * VD_THREADS + tid) * 4, y, 4 * g, a.vocab, y_step);
+                const bool fours = x_step == 4 && y_step == 4;
+                constexpr int ROW = 4 * VD_THREADS, STAGE = 2 * ROW;
+                float* slot = ring + 4 * tid;                // of the stage whose turn it is
+                auto fetch = [&](float* to, int g) {         // NaN where the row has no such tokens
+                    if (fours && 4 * g + 3 < a.vocab) {
+                        copy_16(to, x + 4 * g);
+                        if (failed) copy_16(to + ROW, y + 4 * g);
+                    } else {
+                        copy_four(to, x, 4 * g, a.vocab, x_step);
+                        if (failed) copy_four(to + ROW, y, 4 * g, a.vocab, y_step);
                     }
                     asm volatile("cp.async.commit_group;" ::: "memory");
                 };
@@ -705,44 +714,36 @@ __global__ void __launch_bounds__(VD_THREADS, JUDGED ? 4 : 1) verify_kernel(VdAr
                 // Only tokens whose share can still pass the best B of the block run: share / E > B needs 1 - U < share / B.
                 unsigned beaten = 0u;                        // B as a key, as this warp knows it
                 float spare = INFINITY;                      // 1 / B, with something to spare
+                auto beat = [&](unsigned key) {
+                    beaten = key;
+                    spare = pw.spare() * (failed ? 1.f / key_value(key) : ex2((st.m - key_value(key)) * LOG2E) * st.z);
+                };
 #pragma unroll 1
-                for (int k = 0; k < VD_STAGES; ++k) fetch((rank + k * ctas) * VD_THREADS + tid, k);
-                int stage = 0;
+                for (int k = 0; k < VD_STAGES; ++k) fetch(slot + k * STAGE, (rank + k * ctas) * VD_THREADS + tid);
 #pragma unroll 1
                 for (int g = rank * VD_THREADS + tid; g - tid < groups; g += stride) {
                     asm volatile("cp.async.wait_group %0;" ::"n"(VD_STAGES - 1) : "memory");
-                    const float4 f = *reinterpret_cast<const float4*>(ring + ((stage * 2) * VD_THREADS + tid) * 4);
+                    const float4 f = *reinterpret_cast<const float4*>(slot);
                     float4 o = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
-                    if (failed) o = *reinterpret_cast<const float4*>(ring + ((stage * 2 + 1) * VD_THREADS + tid) * 4);
+                    if (failed) o = *reinterpret_cast<const float4*>(slot + ROW);
                     const float v[4] = {f.x, f.y, f.z, f.w}, q[4] = {o.x, o.y, o.z, o.w};
-                    float p[4], ahead = 0.f;
+                    float p[4];
+                    if (plain) {
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        if (plain) p[i] = ex2(fmaf(fmaxf(v[i], -INFINITY), pw.c, -p2)) - ex2(fmaf(fmaxf(q[i], -INFINITY), pw.c, -q2));
-                        else p[i] = p_of(v[i]) - (failed ? q_of(q[i]) : 0.f);
-                        if (g >= groups) p[i] = 0.f;
-                        ahead = fmaxf(ahead, p[i]);
+                        for (int i = 0; i < 4; ++i) p[i] = ex2(fmaf(fmaxf(v[i], -INFINITY), pw.c, -p2)) - ex2(fmaf(fmaxf(q[i], -INFINITY), pw.c, -q2));
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) p[i] = p_of(v[i]) - (failed ? q_of(q[i]) : 0.f);
                     }
-                    fetch(g + VD_STAGES * stride, stage);    // (what lay there is in registers)
-                    stage = stage + 1 < VD_STAGES ? stage + 1 : 0;
+                    const float ahead = fmaxf(fmaxf(p[0], p[1]), fmaxf(p[2], p[3]));
+                    fetch(slot, g + VD_STAGES * stride);     // (what lay there is in registers)
+                    slot = slot == ring + 4 * tid + (VD_STAGES - 1) * STAGE ? ring + 4 * tid : slot + STAGE;
                     const unsigned now = *reinterpret_cast<volatile unsigned*>(&beat_sh);
-                    if (now != beaten) {
-                        beaten = now;
-                        spare = pw.spare() * (failed ? 1.f / key_value(now) : ex2((st.m - key_value(now)) * LOG2E) * st.z);
-                    }
+                    if (now != beaten) beat(now);
                     if (!__any_sync(~0u, plain ? ahead * spare > 5.9e-8f : ahead > 0.f)) continue;         // 1 - U is 2^-24 at least
                     const uint4 w = philox4x32_10(make_uint4((unsigned)g, c1, stream, domain), key2);
-                    const unsigned words[4] = {w.x, w.y, w.z, w.w};
-                    bool again;
-                    do {
-                        again = plain && spare == INFINITY;  // nothing to beat yet: the foremost of every thread, then all
-                        unsigned run = 0u;
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const bool may = again ? p[i] == ahead : !plain || may_pass(words[i], p[i] * spare);
-                            run |= may && p[i] > 0.f ? 1u << i : 0u;
-                        }
-                        if (!__any_sync(~0u, run)) break;
+                    unsigned run = 0u;
+                    auto run_all = [&]() {
 #pragma unroll 1
                         for (; run; run &= run - 1u) {
                             const int i = __ffs(run) - 1;
@@ -754,10 +755,20 @@ __global__ void __launch_bounds__(VD_THREADS, JUDGED ? 4 : 1) verify_kernel(VdAr
                         const unsigned best = __reduce_max_sync(~0u, b.i < 0 ? 0u : order_key(b.v));
                         if (best > beaten) {
                             if ((tid & 31) == 0) atomicMax(&beat_sh, best);
-                            beaten = best;
-                            spare = pw.spare() * (failed ? 1.f / key_value(best) : ex2((st.m - key_value(best)) * LOG2E) * st.z);
+                            beat(best);
                         }
-                    } while (again && spare != INFINITY);
+                    };
+                    if (spare == INFINITY || !plain) {       // nothing to beat yet: the foremost of every thread first; or no telling: all
+                        const float least = plain ? ahead : 0.f;
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) run |= p[i] > 0.f && p[i] >= least ? 1u << i : 0u;
+                        run_all();
+                        if (!plain) continue;
+                    }
+                    const unsigned words[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) run |= may_pass(words[i], p[i] * spare) ? 1u << i : 0u;
+                    if (__any_sync(~0u, run)) run_all();
                 }
                 asm volatile("cp.async.wait_all;" ::: "memory");
                 b = block_best(b, best_sh);
