@@ -565,6 +565,16 @@ def test_refusals(ops):
         ops.step_arrays(ints([0, 1]), ints([1]), table, rows=4, max_count=2, page_size=8)
 
 
+def test_tensors_of_another_device_than_the_current_one_are_refused(ops, monkeypatch):
+    calls = [lambda: ops.verify_drafts(torch.zeros(2, 9, device=dev()), ints([1, 2]), ints([0, 2]), max_drafts=1),
+             lambda: ops.ngram_drafts(ints([[1, 2]]), ints([2]), max_drafts=1),
+             lambda: ops.step_arrays(ints([0]), ints([1]), ints([[1]]), rows=1, max_count=1, page_size=8)]
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 1)
+    for call in calls:
+        with pytest.raises(ops.KernelError, match="current device is cuda:1"):
+            call()
+
+
 def test_what_the_status_word_says(ops):
     assert "more tokens than its arrays" in ops.status_message(0, 5) and "text has no row" in ops.status_message(0, 6)
     assert "without a page" in ops.status_message(0, 1) and ops.status_message(0, 0) is None

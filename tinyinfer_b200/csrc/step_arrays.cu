@@ -104,8 +104,6 @@ __global__ void __launch_bounds__(SA_THREADS) step_arrays_kernel(SaArgs a) {
 
 }  // namespace
 
-TI_API int ti_step_tile_rows() { return SA_TILE; }
-
 TI_API int ti_step_arrays(int* token_ids, int* positions, int* token_seq, int* cache_slots, int* cu_seqlens, int* q_starts, int* context_lens,
                           int* tiles, int* block_tables, const int* starts, const int* counts, const int* state_slots, const int* tables,
                           const int* tokens, int* status, int requests, int groups, int table_rows, int width, int token_width, int rows,

@@ -14,17 +14,17 @@
 // Sums and exponentials are float32 (the sum over a top-k row's few candidates is taken in fixed point, so that the order in which
 // they were found does not show).
 //
-// Bound by reading the logits once. Three kernels:
+// Bound by reading the logits once. Three kernels (two where every request is greedy):
 //   parts_kernel   streams every row, 32 logits a thread in registers, and leaves of each warp's part the largest, the sum and the best
-//                  draw, or of a top-k row the largest of every 32 neighbouring logits; no block waits for another, no warp for another.
+//                  draw, or of a top-k row the largest of every 32 neighbouring logits. No block waits for another: 64 x 4 rows of
+//                  151,936 and as many of the draft model, less 64, 53 us = 6.6 TB/s; 64 x 7 open ones 86 us = 6.8 TB/s.
 //   rows_kernel    a block a row. Of a top-k row: at least k of the row's lines of 32 reach a value close to the k-th largest of its lines'
 //                  largest, which bounds the row's k-th largest from below; so the row's top k are in the few lines (some 110 for k = 100)
-//                  that reach it, and those are read again and ranked.
-//   verify_kernel  decides the request; behind a drawn draft that failed, clusters of blocks scan the two rows once more.
-// The last two are short: most of their time is the wait for their own instructions (a line of eight that no block of the SM has run yet
-// costs some 240 cycles), so their loops are rolled and what is used twice is a function.
+//                  that reach it, and those are read again and ranked. A chain of short steps on one block: 9 us for one row, 14 for 576.
+//   verify_kernel  decides the request (1 to 2 us); behind a drawn draft that failed, clusters of blocks scan the two rows once more
+//                  (64 requests of 151,936 tokens: 33 us, bound by the Philox words and exponentials of the tokens).
 // A row held by a cluster of 16 blocks in shared memory, threshold and sum found there, read the logits once too, but spent 13 us of a
-// block on meeting the others (a cluster's barrier 0.9 us) where its loads took 1.3: 291 us for 64 x 4 rows of 151,936 with k = 100.
+// block on meeting the others (a cluster's barrier 0.9 us) where its loads took 1.3: 291 us for the first of these cases.
 #include <cooperative_groups.h>
 
 #include <algorithm>
@@ -693,6 +693,7 @@ __global__ void __launch_bounds__(VD_THREADS, JUDGED ? 4 : 1) verify_kernel(VdAr
                 }
             } else {
                 cg::cluster_group cluster = cg::this_cluster();
+                asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");     // this block runs (all of the cluster's come here)
                 extern __shared__ __align__(16) float ring[];                  // [stage][row][thread][4]: a thread's own
                 const int groups = (a.vocab + 3) / 4, ctas = gridDim.x, stride = ctas * VD_THREADS, x_step = row_step(x), y_step = row_step(y);
                 const bool fours = x_step == 4 && y_step == 4;
@@ -772,7 +773,7 @@ __global__ void __launch_bounds__(VD_THREADS, JUDGED ? 4 : 1) verify_kernel(VdAr
                 }
                 asm volatile("cp.async.wait_all;" ::: "memory");
                 b = block_best(b, best_sh);
-                cluster.sync();                              // every block runs
+                asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
                 if (tid == 0) *cluster.map_shared_rank(&part_sh[rank], 0) = b;
                 cluster.sync();
                 if (rank != 0) return;

@@ -32,7 +32,6 @@ _SIGNATURES = {
         "ti_verify_scratch_words": [c_int, c_int, c_int, c_int, c_int],
         "ti_ngram_drafts": [c_void_p] * 11 + [c_int] * 7 + [c_void_p],
         "ti_step_arrays": [c_void_p] * 15 + [c_int] * 9 + [c_void_p],
-        "ti_step_tile_rows": [],
     },
     "core": {
         "ti_embedding": [c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_void_p],
@@ -2434,9 +2433,9 @@ def verify_drafts(logits: torch.Tensor, token_ids: torch.Tensor, cu_rows: torch.
                   stream_id: Optional[torch.Tensor] = None, step: Optional[torch.Tensor] = None,
                   draft_logits: Optional[torch.Tensor] = None) -> VerifiedDrafts:
     """Which drafted tokens hold, and the token behind them. Request r brought the tokens ``token_ids[cu_rows[r] : cu_rows[r + 1]]``
-    (int32 [N]; ``cu_rows`` int32 [S + 1]), one that is settled and up to ``max_drafts`` drafts, and ``logits`` float32 [N, V] (V up to
-    524,288) has the row behind each: row j judges draft j, the last row is for the token behind all of them. Rows past ``max_drafts + 1`` of a request
-    and rows that no request claims are not looked at; a request without rows gets no token.
+    (int32 [N]; ``cu_rows`` int32 [S + 1]), one that is settled and up to ``max_drafts`` (at most 31) drafts, and ``logits`` float32
+    [N, V] (V up to 524,288) has the row behind each: row j judges draft j, the last row is for the token behind all of them. Rows past
+    ``max_drafts + 1`` of a request and rows that no request claims are not looked at; a request without rows gets no token.
 
     The sampling options are those of ``sample``, one entry per request; ``step`` counts for the request's first row, row j draws at
     step + j. Without any of them every request is greedy. Without ``draft_logits`` a draft holds where it is the token that ``sample``
