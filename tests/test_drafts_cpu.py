@@ -151,3 +151,21 @@ def test_status_words():
     from tinyinfer_b200 import ops
     assert "more tokens than its arrays" in ops.status_message(0, 5) and "text has no row" in ops.status_message(0, 6)
     assert "without a page" in ops.status_message(0, 1) and ops.status_message(0, 0) is None
+
+
+@pytest.mark.parametrize("kw", [dict(rows=1 << 30), dict(rows=1 << 32), dict(max_count=1 << 30), dict(max_count=(1 << 32) + 2),
+                                dict(page_size=1 << 32), dict(page_size=(1 << 32) + 8), dict(pad_page=1 << 31)])
+def test_sizes_that_pass_32_bits_are_refused(ops, kw):
+    with pytest.raises(ops.KernelError, match="bad sizes"):
+        ops.step_arrays(i32(0, 1), i32(1, 1), i32(1, 2, 3, 4).view(2, 2), **dict(dict(rows=4, max_count=2, page_size=8), **kw))
+    assert not ops.calls
+
+
+def test_a_status_without_a_word_or_of_another_device_is_refused(ops):
+    table, h = i32(1, 2, 3, 4).view(2, 2), torch.zeros(2, 8, dtype=torch.int32)
+    for status in (i32(), torch.zeros(1, dtype=torch.int32, device="meta")):
+        with pytest.raises(ops.KernelError):
+            ops.step_arrays(i32(0, 1), i32(1, 1), table, rows=4, max_count=2, page_size=8, status=status)
+        with pytest.raises(ops.KernelError):
+            ops.ngram_drafts(h, i32(3, 4), max_drafts=2, status=status)
+    assert not ops.calls

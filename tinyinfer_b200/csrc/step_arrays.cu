@@ -110,7 +110,7 @@ TI_API int ti_step_arrays(int* token_ids, int* positions, int* token_seq, int* c
                           int max_count, int page_size, int pad_page, cudaStream_t stream) {
     TI_REQUIRE(requests >= 0 && requests < 65535 && groups >= 1 && table_rows >= 0 && width >= 1 && rows >= 0 && max_count >= 1 && page_size >= 1,
                "step_arrays: bad sizes");
-    TI_REQUIRE(rows <= (1 << 30) && max_count <= (1 << 30), "step_arrays: at most 2^30 rows");
+    TI_REQUIRE(rows < (1 << 30) && max_count < (1 << 30), "step_arrays: fewer than 2^30 rows");     // two of them add up to less than 2^31
     TI_REQUIRE((token_ids == nullptr) == (tokens == nullptr) && (!tokens || token_width >= max_count), "step_arrays: tokens narrower than max_count");
     SaArgs a{starts, counts, state_slots, tables, tokens, token_ids, positions, token_seq, cache_slots, cu_seqlens, q_starts, context_lens,
              (int4*)tiles, block_tables, status, requests, groups, table_rows, width, token_width, rows, max_count,

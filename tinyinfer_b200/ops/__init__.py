@@ -2400,6 +2400,13 @@ def _per_request(t: torch.Tensor, name: str, dtype, n: int, device) -> None:
         raise KernelError(f"{name} lies on {t.device}, the others on {device}")
 
 
+def _check_word(t: torch.Tensor, name: str, device) -> None:
+    """Checks a tensor whose first entry a kernel may write."""
+    _check(t, name, torch.int32, 1)
+    if t.shape[0] < 1 or t.device != device:
+        raise KernelError(f"{name} must have an entry on {device}, got {t.shape[0]} on {t.device}")
+
+
 _layouts = {}
 _NO_OPTIONS = (None,) * 6
 _SCRATCH_BEHIND = 1 << 18     # words of scratch (1 MB) that may lie behind a call's outputs
@@ -2456,7 +2463,7 @@ def verify_drafts(logits: torch.Tensor, token_ids: torch.Tensor, cu_rows: torch.
     _check(cu_rows, "cu_rows", torch.int32, 1)
     n, vocab = logits.shape
     s, d, device = cu_rows.shape[0] - 1, int(max_drafts), logits.device
-    if s < 0 or token_ids.shape[0] != n or vocab < 1:
+    if s < 0 or token_ids.shape[0] != n or vocab < 1 or n >= 1 << 31:
         raise KernelError(f"verify_drafts: {tuple(logits.shape)} logits, {token_ids.shape[0]} tokens, cu_rows of {s + 1} entries")
     if not 0 <= d <= MAX_DRAFTS:
         raise KernelError(f"verify_drafts: max_drafts must be 0 to {MAX_DRAFTS}, got {d}")
@@ -2549,7 +2556,7 @@ def ngram_drafts(history: torch.Tensor, lengths: torch.Tensor, *, max_drafts: in
     if limits is not None:
         _per_request(limits, "limits", torch.int32, s, device)
     if status is not None:
-        _check(status, "status", torch.int32, 1)
+        _check_word(status, "status", device)
     stream = _stream_of(device)
     out = NgramDrafts(*_packed(device, (s, d + 1), (s,), (s,), (s,))[:4])
     _run("drafts", "ti_ngram_drafts", out.tokens.data_ptr(), out.counts.data_ptr(), out.starts.data_ptr(), out.lengths.data_ptr(),
@@ -2566,7 +2573,7 @@ def step_arrays(starts: torch.Tensor, counts: torch.Tensor, block_tables: torch.
     ``token_ids`` are made). ``block_tables`` int32 [groups, M, width] (or [M, width]: one group) holds the pages of every request,
     request s's in row ``state_slots[s]`` (int32 [S]; None: row s): as many as its tokens need, -1 where it has none.
 
-    The result has ``rows`` flat rows, whatever the counts: the requests' tokens one after the other, and behind them rows of a
+    The result has ``rows`` flat rows (as ``max_count`` fewer than 2^30), whatever the counts: the requests' tokens one after the other, and behind them rows of a
     request number S at position 0 with the one page ``pad_page``, which no other request holds (-1: none), so that a step of a fixed size
     can be captured. Their ``cache_slots`` are -1. ``cu_seqlens``: the requests' first rows, that of number S, ``rows``. ``tiles``: up to
     128 rows each, ``ceil(max_count / 128)`` per request, [request, first row, rows (0: none), first position], as the one-tile attention
@@ -2589,15 +2596,15 @@ def step_arrays(starts: torch.Tensor, counts: torch.Tensor, block_tables: torch.
                           f"{block_tables.device}")
     if state_slots is None and table_rows < s:
         raise KernelError(f"step_arrays: {s} requests, but the block tables have {table_rows} rows")
-    if rows < 0 or max_count < 1 or page_size < 1:
-        raise KernelError(f"step_arrays: bad sizes: rows {rows}, max_count {max_count}, page_size {page_size}")
+    if not (0 <= rows < 1 << 30 and 1 <= max_count < 1 << 30 and 1 <= page_size < 1 << 31 and -(1 << 31) <= pad_page < 1 << 31):
+        raise KernelError(f"step_arrays: bad sizes: rows {rows}, max_count {max_count}, page_size {page_size}, pad_page {pad_page}")
     if tokens is not None:
         _check(tokens, "tokens", torch.int32, 2)
         if tokens.shape[0] != s or tokens.shape[1] < max_count or tokens.device != device:
             raise KernelError(f"step_arrays: tokens must be [{s}, at least {max_count}] on {device}, got {tuple(tokens.shape)} on "
                               f"{tokens.device}")
     if status is not None:
-        _check(status, "status", torch.int32, 1)
+        _check_word(status, "status", device)
     stream = _stream_of(device)
     tiles = s * -(-max_count // STEP_TILE)
     shapes = ((rows,), (rows,), (groups, rows), (s + 2,), (s + 1,), (s + 1,), (tiles, 4), (groups, s + 1, width))
