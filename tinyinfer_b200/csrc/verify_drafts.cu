@@ -739,7 +739,8 @@ __global__ void __launch_bounds__(VD_THREADS, JUDGED ? 4 : 1) verify_kernel(VdAr
                     const float ahead = fmaxf(fmaxf(p[0], p[1]), fmaxf(p[2], p[3]));
                     fetch(slot, g + VD_STAGES * stride);     // (what lay there is in registers)
                     slot = slot == ring + 4 * tid + (VD_STAGES - 1) * STAGE ? ring + 4 * tid : slot + STAGE;
-                    const unsigned now = *reinterpret_cast<volatile unsigned*>(&beat_sh);
+                    // (one lane's view for all: another warp may write between two lanes' reads, and what follows is the warp's as a whole)
+                    const unsigned now = __shfl_sync(~0u, *reinterpret_cast<volatile unsigned*>(&beat_sh), 0);
                     if (now != beaten) beat(now);
                     if (!__any_sync(~0u, plain ? ahead * spare > 5.9e-8f : ahead > 0.f)) continue;         // 1 - U is 2^-24 at least
                     const uint4 w = philox4x32_10(make_uint4((unsigned)g, c1, stream, domain), key2);
