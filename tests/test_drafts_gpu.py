@@ -529,6 +529,61 @@ def test_arrays_that_do_not_fit(ops):
     assert none.token_seq.tolist() == [0, 0] and none.cu_seqlens.tolist() == [0, 2] and none.block_tables.tolist() == [[[9, -1]]]
 
 
+# ------------------------------------------------------------------------------------------------ all three
+def test_offsets_that_pass_32_bits(ops):
+    """Logits, draft logits, texts and tables of more than 2^31 elements, of which only the last are looked at."""
+    buf = torch.empty((1 << 31) + (1 << 22), dtype=torch.int32, device=dev())          # 8.6 GB
+    counts, vocab = [4, 2, 4], 32003
+    logits, fed = batch(counts, vocab, seed=71)
+    q = near(logits, counts, 3, 71)
+    opts = options(3, 71, topk=[0, 20, 0])
+    want = check(ops, logits, fed, counts, 3, opts, q)
+    rows = buf.numel() // vocab
+    far = buf[:rows * vocab].view(rows, vocab).view(torch.float32)
+    far[-10:] = logits
+    far_fed = torch.zeros(rows, dtype=torch.int32, device=dev())
+    far_fed[-10:] = ints(fed)
+    cu = ints([rows - 10 + c for c in rows_of(counts)])
+    got = ops.verify_drafts(far, far_fed, cu, max_drafts=3, draft_logits=q, **opts)
+    assert all(torch.equal(x, y) for x, y in zip(got, want))
+    # draft logits whose requests, then whose drafts, lie 2^29 and more elements apart
+    for strides in ((1 << 30, 1 << 18, 1), (1 << 18, 1 << 30, 1)):
+        far_q = buf.view(torch.float32).as_strided((3, 3, vocab), strides, 1 << 20)
+        assert 2 * (1 << 30) + 2 * (1 << 18) + (1 << 20) + vocab <= buf.numel()
+        far_q.copy_(q)
+        got = ops.verify_drafts(logits, ints(fed), ints(rows_of(counts)), max_drafts=3, draft_logits=far_q, **opts)
+        assert all(torch.equal(x, y) for x, y in zip(got, want))
+    # texts
+    room = 1 << 20
+    rows = buf.numel() // room
+    history = buf[:rows * room].view(rows, room)
+    history[-1, :5] = ints([4, 8, 15, 4, 8])
+    got = ops.ngram_drafts(history, ints([5]), max_drafts=2, state_slots=ints([rows - 1]), tokens=ints([[15, 4]]), counts=ints([2]))
+    assert got.tokens.tolist() == [[4, 8, 15]] and history[-1, :7].tolist() == [4, 8, 15, 4, 8, 15, 4]
+    # tables of two groups
+    rows = buf.numel() // 2048
+    tables = buf[:rows * 2048].view(2, rows // 2, 1024 * 2)
+    tables[0, -1, :3], tables[1, -1, :3] = ints([5, 6, 7]), ints([8, 9, 10])
+    got = ops.step_arrays(ints([30]), ints([3]), tables, rows=3, max_count=3, page_size=16, state_slots=ints([rows // 2 - 1]))
+    assert got.cache_slots.tolist() == [[6 * 16 + 14, 6 * 16 + 15, 7 * 16], [9 * 16 + 14, 9 * 16 + 15, 10 * 16]]
+    assert got.block_tables[:, 0, :4].tolist() == [[5, 6, 7, -1], [8, 9, 10, -1]]
+
+
+def test_requests_that_share_what_they_read(ops):
+    """Texts and tables by the same slot twice (nothing is brought, so nothing is written), draft logits of one row for all."""
+    history = ints([[9] * 8, [1, 2, 3, 1, 2, 3, 1, 0]])
+    got = ops.ngram_drafts(history, ints([7, 5, 7]), max_drafts=3, state_slots=ints([1, 1, 1]))
+    assert got.tokens.tolist() == [[1, 2, 3, 1], [2, 3, 1, 2], [1, 2, 3, 1]]
+    arrays_check(ops, [0, 9, 0], [3, 4, 3], [[[3, 4, 5], [7, 8, 9]]], rows=12, max_count=4, page_size=8, state_slots=[1, 1, 1], pad_page=2)
+    counts = [3, 2, 4]
+    logits, fed = batch(counts, 2500, seed=72)
+    q = (2.0 * torch.randn(2500, generator=torch.Generator().manual_seed(73))).to(dev())
+    opts = options(3, 72, topk=[0, 30, 0])
+    a = check(ops, logits, fed, counts, 3, opts, q.expand(3, 3, 2500))
+    b = ops.verify_drafts(logits, ints(fed), ints(rows_of(counts)), max_drafts=3, draft_logits=q.expand(3, 3, 2500).contiguous(), **opts)
+    assert all(torch.equal(x, y) for x, y in zip(a, b))
+
+
 # ------------------------------------------------------------------------------------------------ refusals
 def test_refusals(ops):
     logits, fed, cu = torch.zeros(4, 9, device=dev()), ints([1, 2, 3, 4]), ints([0, 2, 4])
