@@ -123,9 +123,9 @@ struct Weights {
 // The same of a scaled logit at hand.
 __device__ __forceinline__ float scaled_weight(float s, float m) { return !(s > -INFINITY) ? 0.f : (s == m ? 1.f : ex2((s - m) * LOG2E)); }
 
-// Whether 1 - U < x for the uniform number U of a word of the stream. 1 - U is (2^23 - 1 - word / 2^9) / 2^23 + 2^-24, exactly; the first
-// summand is had from the word's bits by one subtraction.
-__device__ __forceinline__ bool may_pass(unsigned word, float x) { return 1.99999988f - __uint_as_float(0x3F800000u | word >> 9) < x - 5.9604645e-8f; }
+// Whether 1 - U < x * y may hold for the uniform number U of a word of the stream (never no where it does). 1 - U is 2 - 2^-24 - f, f the
+// float in [1, 2) with the word's upper bits; so f + x y > 2 - 2^-24, which rounds to 2 at least, as the tie does.
+__device__ __forceinline__ bool may_pass(unsigned word, float x, float y) { return fmaf(x, y, __uint_as_float(0x3F800000u | word >> 9)) >= 2.f; }
 
 // s + G of a scaled logit s and its uniform number.
 __device__ __forceinline__ float noisy(float s, float u) { return s - logf(-logf(u)); }
@@ -278,19 +278,32 @@ __global__ void __launch_bounds__(VD_THREADS, DRAWS ? 4 : 5) parts_kernel(VdArgs
 #pragma unroll 1
         for (int half = 0; half < 2; ++half) {               // the threads' largest logits for a first B, then all
             unsigned left = 0u;
+            if (half == 0) {
 #pragma unroll
-            for (int k = 0; k < VD_GROUPS; ++k) {
-                if (half == 0) {
+                for (int k = 0; k < VD_GROUPS; ++k)
 #pragma unroll
                     for (int q = 0; q < 4; ++q) left = v[k][q] == most ? 1u << (4 * k + q) : left;
-                } else {
-                    uint2 key = key2;                        // its ten bumps are made anew for every block: kept, they cost twenty registers
-                    asm volatile("" : "+r"(key.x), "+r"(key.y));
-                    const uint4 w = philox4x32_10(make_uint4((unsigned)token_of(blockIdx.x, tid, k) >> 2, c1, stream, 0u), key);
-                    const unsigned words[4] = {w.x, w.y, w.z, w.w};
+            } else {
+                // round by round for all groups: they share the key's bumps and what the first rounds make of the step and the stream
+                // (320 open rows of 151,936 looked-up drafts 94 us; group by group 104)
+                uint2 key = key2;
+                asm volatile("" : "+r"(key.x), "+r"(key.y));             // bumped here, not ahead: that would take twenty registers
+                uint4 w[VD_GROUPS];
+#pragma unroll
+                for (int k = 0; k < VD_GROUPS; ++k) w[k] = make_uint4((unsigned)token_of(blockIdx.x, tid, k) >> 2, c1, stream, 0u);
+#pragma unroll
+                for (int round = 0; round < 10; ++round) {
+#pragma unroll
+                    for (int k = 0; k < VD_GROUPS; ++k) w[k] = philox_round(w[k], key);
+                    key.x += 0x9E3779B9u;
+                    key.y += 0xBB67AE85u;
+                }
+#pragma unroll
+                for (int k = 0; k < VD_GROUPS; ++k) {
+                    const unsigned words[4] = {w[k].x, w[k].y, w[k].z, w[k].w};
 #pragma unroll
                     for (int q = 0; q < 4; ++q)
-                        left |= (weight.odd ? v[k][q] > -INFINITY : may_pass(words[q], v[k][q] * spare)) ? 1u << (4 * k + q) : 0u;
+                        left |= (weight.odd ? v[k][q] > -INFINITY : may_pass(words[q], v[k][q], spare)) ? 1u << (4 * k + q) : 0u;
                 }
             }
             if (half == 0 && !(most > (weight.odd ? -INFINITY : 0.f))) left = 0u;       // (a weight of nothing is beaten by the largest)
@@ -769,7 +782,7 @@ __global__ void __launch_bounds__(VD_THREADS, JUDGED ? 4 : 1) verify_kernel(VdAr
                     }
                     const unsigned words[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) run |= may_pass(words[i], p[i] * spare) ? 1u << i : 0u;
+                    for (int i = 0; i < 4; ++i) run |= may_pass(words[i], p[i], spare) ? 1u << i : 0u;
                     if (__any_sync(~0u, run)) run_all();
                 }
                 asm volatile("cp.async.wait_all;" ::: "memory");
