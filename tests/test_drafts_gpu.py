@@ -219,6 +219,16 @@ def test_thresholds_in_the_thousands(ops, with_q):
           may_skip=0.3)
 
 
+@pytest.mark.parametrize("vocab", [2500, 40007])
+@pytest.mark.parametrize("with_q", [False, True])
+def test_thresholds_in_the_hundreds(ops, vocab, with_q):
+    ks = [255, 256, 383, 384, 385, 450, 511, 512, 513, 700, 1023, 1500]
+    counts = [3] * len(ks)
+    logits, fed = batch(counts, vocab, seed=vocab + 1)
+    logits[4] = torch.round(logits[4])                       # many equal ones, at the threshold too
+    check(ops, logits, fed, counts, 2, options(len(ks), vocab, topk=ks), near(logits, counts, 2, vocab) if with_q else None)
+
+
 def test_many_requests_and_the_largest_vocabulary(ops):
     rng = np.random.RandomState(4)
     counts = rng.randint(0, 4, 400).tolist()

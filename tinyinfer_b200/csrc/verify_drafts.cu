@@ -409,17 +409,21 @@ __device__ __noinline__ unsigned reached_by(unsigned one, unsigned two, bool pai
     return lo;
 }
 
-// The same for any number of lines, by halving over all of them: a k in the hundreds.
-__device__ __noinline__ unsigned lines_reached_by(RowShared& sh, const float* largest, int n, int k) {
-    unsigned lo = order_key(-INFINITY), hi = order_key(INFINITY);     // at least k reach lo
+// The same for any number of lines, none of which passes hi, by halving over all of them: a k in the hundreds.
+__device__ __noinline__ unsigned lines_reached_by(RowShared& sh, const float* largest, int n, unsigned hi, int k, int spare) {
+    unsigned lo = order_key(-INFINITY);                               // at least k reach lo
 #pragma unroll 1
     for (int i = 0; i < 20 && lo < hi; ++i) {
         const unsigned middle = lo + (hi - lo + 1) / 2;
         int reach = 0;
         for (int j = threadIdx.x; j < n; j += VD_THREADS) reach += order_key(largest[j]) >= middle;
         reach = (int)block_sum((float)reach, sh.red);                 // at most 2^14 of them: exact
-        if (reach >= k) lo = middle;
-        else hi = middle - 1;
+        if (reach < k) {
+            hi = middle - 1;
+        } else {
+            lo = middle;
+            if (reach <= k + spare) break;
+        }
     }
     return lo;
 }
@@ -507,8 +511,10 @@ __global__ void __launch_bounds__(VD_THREADS, 4) rows_kernel(VdArgs a) {
         if (i + VD_THREADS < n_lines) two = fmaxf(two, largest[i + VD_THREADS]);
     }
     const Range offered = key_range(order_key(one), order_key(two), sh.range);
-    const unsigned bound = topk <= 2 * VD_THREADS ? reached_by(order_key(one), order_key(two), true, offered.least, offered.most, topk, topk / 8)
-                                                  : lines_reached_by(sh, largest, n_lines, topk);
+    // (near a k of all 512 shares their k-th largest is their least, which far too many lines reach: 64 x 3 rows and as many of the draft
+    // model by the shares, by all lines, k = 100: 60, 78 us; k = 350: 79, 88 us; k = 400: 86, 88 us; k = 450: 414, 92 us)
+    const unsigned bound = topk <= VD_THREADS * 3 / 2 ? reached_by(order_key(one), order_key(two), true, offered.least, offered.most, topk, topk / 8)
+                                                      : lines_reached_by(sh, largest, n_lines, offered.most, topk, topk / 8);
     // (What lies 110 below the largest, scaled, has no weight in float32 and no noise that makes up for it: the tokens that a mask of the
     // type's lowest value leaves behind its own are not candidates, though the threshold may not drop them.)
     const float most = key_value(offered.most), floor = fabsf(most / temp) < 1e30f ? most - 110.f * temp : -INFINITY;
@@ -591,9 +597,7 @@ __global__ void __launch_bounds__(VD_THREADS, 4) rows_kernel(VdArgs a) {
             }
         };
         if (n >= topk) st.threshold = select_kth(topk, sh.hist, sh.sel, [&](auto count) { each([&](float s, int) { count(score_key(s)); }); });
-        float largest_scaled = -INFINITY;
-        each([&](float s, int) { largest_scaled = fmaxf(largest_scaled, s); });
-        st.m = block_max(largest_scaled, sh.red);
+        st.m = most / temp;                                  // (quotients keep the order of what is divided)
         if (!fits) {
             each([&](float s, int token) { take(s, token); });
             if (tid == 0) sh.listed = a.list + 1;
