@@ -1,0 +1,171 @@
+"""Verification of drafts where the logits lie far from 0: masks of a large negative number, which float32 still divides by the
+temperature, rows that lie there as a whole, and temperatures near 0."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+import plain_drafts as plain
+
+pytestmark = pytest.mark.gpu
+NAMES = ("temperature", "topk", "greedy", "seed", "stream_id", "step")
+
+
+def dev():
+    return torch.device("cuda:0")
+
+
+@pytest.fixture(scope="module")
+def ops():
+    from tinyinfer_b200 import ops
+    return ops
+
+
+def ints(values, dtype=torch.int32):
+    return torch.tensor(values, dtype=dtype, device=dev())
+
+
+def options(temperature, topk, seed):
+    s = len(temperature)
+    g = torch.Generator().manual_seed(seed)
+    return dict(temperature=torch.tensor(temperature, dtype=torch.float32, device=dev()), topk=ints(topk), greedy=ints([0] * s),
+                seed=torch.randint(0, 1 << 60, (s,), generator=g).to(dev()),
+                stream_id=torch.randint(0, 1 << 30, (s,), generator=g).to(torch.int32).to(dev()),
+                step=torch.randint(0, 100000, (s,), generator=g).to(torch.int32).to(dev()))
+
+
+def sizes(row, temperature, topk):
+    """How large the scaled logits are that have weight (they lie within 110 of the largest), and whether they differ."""
+    s = plain.scaled(row, temperature, topk)
+    near = s[s >= s.max() - 110.0] if s.max() > -math.inf else s[:0]
+    near = near[np.isfinite(near)]
+    return (float(np.abs(near).max()), bool((near != near[0]).any())) if near.size else (0.0, False)
+
+
+def tolerances(rows, temperature, topk):
+    """(of a probability's ratio, relative; of a draw's lead).
+    A row without a threshold weighs its logits by their distance from the largest, up to 110 / ln 2 = 159 in powers of two: the
+    difference, the factor (two roundings) and the product are half a step (2^-24) each, the exponential four steps of 2^-24, the sum a
+    half step for each addition of a thread and of the tree (vocab / 256 + 16). With a threshold the scaled logits are subtracted, each
+    a half step off at its own size, where they differ. A ratio has all that twice, and a division. A score s + G has the quotient's half
+    step and the sum's at the size of s, and 2^-19 of G (at most 17, two logarithms of a few steps)."""
+    size, extra = 0.0, 0.0
+    for row in rows:
+        largest, differ = sizes(row, temperature, topk)
+        size = max(size, largest)
+        if differ and 0 < topk < row.shape[0]:
+            extra = max(extra, largest)
+    vocab = rows[0].shape[0]
+    rel = 2 * 2.0 ** -24 * (4 * 159 * math.log(2) + 4 * extra + 8 + vocab / 256 + 16) + 2.0 ** -23
+    return rel, 2 * (2 * 2.0 ** -24 * size + 2.0 ** -19)
+
+
+def leftover_is_decided(row, dl, rel, temperature, topk, seed, stream, step):
+    """Whether float32 can tell which token the draw behind a failed draft gives. What is left of p beyond q is a difference: it is known
+    to rel (p + q) and to 2^-126, below which a probability is nothing. (Where p and q are 1 but for 1e-66 the formula has tokens left
+    of which float32 has none, and p itself is drawn from.)"""
+    p, q = (plain.probabilities(plain.scaled(v, temperature, topk)) for v in (row, dl))
+    left, off = np.maximum(p - q, 0.0), rel * (p + q) + 2.0 ** -126
+    race = -np.log(-np.log(plain.uniforms(row.shape[0], step, stream, 2, seed)))
+    with np.errstate(divide="ignore"):
+        least, most = np.log(np.maximum(left - off, 0.0)) + race, np.log(left + off) + race
+    winner = int(np.argmax(np.log(left + 1e-300) + race))
+    return least[winner] > np.delete(most, winner).max()
+
+
+def check(ops, x, fed, opts, q=None, allowed=None):
+    """x [S, 2, V]: a draft each. The operator beside the plain statement in 64 bits; returns how many requests' tokens were compared
+    (where two scores lie closer than float32 tells apart, they are not)."""
+    s, _, vocab = x.shape
+    got = ops.verify_drafts(x.reshape(2 * s, vocab), ints(fed).flatten(), ints(range(0, 2 * s + 1, 2)), max_drafts=1, draft_logits=q, **opts)
+    tokens, counts, accept = got.tokens.tolist(), got.counts.tolist(), got.accept.cpu().double().numpy()
+    assert np.isfinite(accept).all() and (accept >= 0).all()
+    host, compared = {n: t.tolist() for n, t in opts.items()}, 0
+    for r in range(s):
+        rows = x[r].cpu().numpy()
+        dl = None if q is None else q[r].cpu().numpy()
+        t, k = host["temperature"][r], host["topk"][r]
+        want, acc, margin = plain.verify(rows, fed[r], max_drafts=1, draft_logits=dl, temperature=t, topk=k, greedy=False,
+                                         seed=host["seed"][r], stream=host["stream_id"][r], step=host["step"][r])
+        rel, lead = tolerances(list(rows) + ([] if dl is None else list(dl)), t, k)
+        assert abs(accept[r, 0] - acc[0]) <= rel * acc[0] + 1e-37, (r, t, k, accept[r, 0], acc[0])
+        assert 1 <= counts[r] <= 2 and all(0 <= i < vocab for i in tokens[r][:counts[r]]) and tokens[r][counts[r]:] == [-1] * (2 - counts[r])
+        if allowed is not None and allowed[r] is not None:
+            assert all(i in allowed[r] for i in tokens[r][:counts[r]]), (r, t, k, tokens[r])
+        decided = margin > 2 * rel + lead
+        if decided and dl is not None and len(want) == 1:
+            decided = leftover_is_decided(rows[0], dl[0], rel, t, k, host["seed"][r], host["stream_id"][r], host["step"][r])
+        if decided:
+            compared += 1
+            assert tokens[r][:counts[r]] == want, (r, t, k, tokens[r], want, margin)
+    return compared
+
+
+TEMPERATURES = [0.3, 0.45, 0.6, 0.7, 0.9, 1.0, 1.3, 1.5]
+
+
+@pytest.mark.parametrize("mask", [-1e4, -1e9, -1e10, -1e15, -1e20, -1e30, -1e38])
+@pytest.mark.parametrize("topk", [0, 20])
+def test_rows_masked_by_a_large_negative_number(ops, mask, topk):
+    """A few tokens allowed, side by side or far apart, half of the vocabulary, all but one; looked-up drafts and drawn ones, against draft
+    logits under the same mask and without; drafts that the mask forbids never hold."""
+    vocab = 20011
+    g = torch.Generator().manual_seed(5)
+    some = [[40, 41, 42], [3, 9000, 20010], list(range(10000)), [i for i in range(vocab) if i != 77]]
+    temperature = TEMPERATURES * len(some)
+    s = len(temperature)
+    x, allowed, fed = torch.full((s, 2, vocab), mask), [], []
+    for r in range(s):
+        own = some[r // len(TEMPERATURES)]
+        x[r][:, own] = 3.0 * torch.randn(2, len(own), generator=g)
+        allowed.append(set(own))
+        likely = own[int(x[r, 0, own].argmax())]
+        fed.append([1, 77 if r % 3 == 0 else likely])    # (77 is forbidden by all masks but the third)
+    x = x.to(dev())
+    opts = options(temperature, [topk] * s, seed=int(-math.log10(-mask)) + 60)
+    open_q = (2.0 * torch.randn(s, 1, vocab, generator=g)).to(dev())
+    like_q = torch.where(x[:, :1] == mask, x[:, :1], x[:, :1] + 0.7 * torch.randn(s, 1, vocab, generator=g).to(dev()))
+    for q in (None, open_q, like_q):
+        assert check(ops, x, fed, opts, q, allowed) >= s // 2
+    # every request's draft forbidden: none holds, and none is written
+    forbidden = [[1, next(i for i in range(vocab) if i not in a)] for a in allowed]
+    for q in (None, open_q):
+        check(ops, x, forbidden, opts, q, allowed)
+
+
+@pytest.mark.parametrize("mask", [-1e4, -1e9, -1e10, -1e15, -1e20, -1e30, -1e38])
+@pytest.mark.parametrize("topk", [0, 20])
+def test_rows_that_lie_at_the_mask_as_a_whole(ops, mask, topk):
+    """Every token alike: a probability of 1 / V each; what is drawn is what sample draws."""
+    vocab, s = 9001, len(TEMPERATURES)
+    x = torch.full((s, 2, vocab), mask, device=dev())
+    opts = options(TEMPERATURES, [topk] * s, seed=7)
+    drawn = ops.sample(x[:, 0].contiguous(), *(opts[n] for n in NAMES)).tolist()
+    fed = [[1, drawn[r] if r % 2 else (drawn[r] + 1) % vocab] for r in range(s)]
+    check(ops, x, fed, opts)
+    got = ops.verify_drafts(x.view(2 * s, vocab), ints(fed).flatten(), ints(range(0, 2 * s + 1, 2)), max_drafts=1, **opts)
+    assert got.tokens[:, 0].tolist() == drawn and got.counts.tolist() == [1 + r % 2 for r in range(s)]
+    check(ops, x, fed, opts, x[:, :1])                   # the same logits: every draft holds
+    check(ops, x, fed, opts, torch.randn(s, 1, vocab, generator=torch.Generator().manual_seed(3)).to(dev()))
+
+
+COLD = [1e-2, 1e-3, 1e-4, 1e-5, 1e-6, 1e-7, 1e-8, 1e-10, 1e-15, 1e-20, 1e-25, 1e-29, 1e-31]
+
+
+@pytest.mark.parametrize("shift", [0.0, 30.0, -1000.0])
+@pytest.mark.parametrize("topk", [0, 20])
+def test_temperatures_near_0(ops, shift, topk):
+    """The largest logit has all the weight, or shares it with its equals."""
+    vocab, s = 20011, len(COLD)
+    g = torch.Generator().manual_seed(9)
+    x = shift + 3.0 * torch.randn(s, 2, vocab, generator=g)
+    best = x[:, 0].argmax(1).tolist()
+    fed = [[1, best[r] if r % 4 else (best[r] + 5) % vocab] for r in range(s)]
+    x[2::3, 0, 19000:19003] = x[2::3, 0].amax(1)[:, None]           # of several equals each has its share
+    x = x.to(dev())
+    opts = options(COLD, [topk] * s, seed=11)
+    # (a draw among equals whose noise is lost beside s is left to the comparison with sample)
+    assert check(ops, x, fed, opts) >= s // 3
+    for q in (x[:, :1], x[:, :1] + 0.5 * torch.randn(s, 1, vocab, generator=g).to(dev())):
+        check(ops, x, fed, opts, q)

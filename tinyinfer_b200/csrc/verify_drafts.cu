@@ -12,7 +12,8 @@
 //   it is that one. That is as likely as rejection sampling makes it, p(d), and the tokens are those of decoding one by one.
 // Greedy requests draw the first largest logit.
 // Sums and exponentials are float32 (the sum over a top-k row's few candidates is taken in fixed point, so that the order in which
-// they were found does not show).
+// they were found does not show). The threshold and the draws go by the float32 quotients s; the weights of a row without a threshold go
+// by x - max x, which comes closer to the softmax of x / T where logits or reciprocal temperatures are large.
 //
 // Bound by reading the logits once. Three kernels (two where every request is greedy):
 //   parts_kernel   streams every row, 32 logits a thread in registers, and leaves of each warp's part the largest, the sum and the best
@@ -48,9 +49,9 @@ constexpr int VD_CTAS = 8, VD_MOST_CTAS = 16;         // blocks that share such 
 constexpr int VD_STAGES = 3;         // groups of four tokens on their way to a thread there
 constexpr float LOG2E = 1.4426950408889634f;
 
-// A warp's part of a row: the largest scaled logit, the sum of the exponentials relative to it, the best draw.
+// A warp's part of a row: the largest logit, the sum of the weights relative to it, the best draw.
 struct __align__(16) Part { float m, z, v; int i; };
-// A row: the largest scaled logit, the sum of the kept exponentials, the lowest kept key, the token that it draws (-1: none; of a
+// A row: the largest logit, the sum of the kept weights, the lowest kept key, the token that it draws (-1: none; of a
 // sampled row that a draft model's logits judge: not drawn), the share of its draft, how many kept tokens are listed (-1: not).
 struct __align__(16) RowStats { float m, z; unsigned threshold; int drawn; float share; int listed, unused[2]; };
 struct __align__(8) Kept { float s; int i; };
@@ -103,20 +104,26 @@ __device__ __forceinline__ float ex2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
-// The weights of a row's logits, exp(v / temp - m): 2^(v * c - m * log2 e), one multiply-add and one exponential. Where that has
-// infinities on both sides (an infinite logit; a temperature whose quotients leave float32) the quotient itself is compared.
+// The weights of a row's logits by their distance from the largest, `most`: exp((v - most) / temp), which is 1 at the largest however far
+// the logits lie from 0 (a mask's -1e10, a temperature near 0): an error in (v - most) c is one of the distance alone. Where a quotient
+// is infinite, or the temperature's reciprocal nearly, the quotients themselves are compared.
+// `fast`, for many logits at once, is one multiply-add and one exponential, 2^(v c - m2) with m2 = most c rounded: that is 2^lost off,
+// alike for all, and lost is an exact float32. At |m| < 2^20 (`near`) it is 0.09 at most; beyond, it may be anything (2^440 at -1e10).
+constexpr float NEAR = 1048576.f;
 struct Weights {
-    float temp, m, c, m2;
+    float temp, most, m, c, m2;
     bool odd;
-    __device__ __forceinline__ Weights(float temp_, float m_) : temp(temp_), m(m_), c(LOG2E / temp_), m2(m_ * LOG2E) {
-        odd = !(fabsf(m) < 1e30f) || !(c < 1e30f);
+    __device__ __forceinline__ Weights(float temp_, float most_) : temp(temp_), most(most_), m(most_ / temp_), c(LOG2E / temp_), m2(most_ * c) {
+        odd = !(fabsf(m) < INFINITY) || !(c < 1e30f);
     }
+    __device__ __forceinline__ bool near() const { return fabsf(m) < NEAR; }
+    __device__ __forceinline__ float lost() const { return fmaf(most, c, -m2); }
     __device__ __forceinline__ float fast(float v) const { return ex2(fmaf(v, c, -m2)); }
     __device__ __forceinline__ float quotient(float v) const {
         const float s = v / temp;
         return !(s > -INFINITY) ? 0.f : (s == m ? 1.f : expf(s - m));
     }
-    __device__ __forceinline__ float operator()(float v) const { return odd ? quotient(v) : fast(v); }
+    __device__ __forceinline__ float operator()(float v) const { return odd ? quotient(v) : ex2((v - most) * c); }
     // A factor on the weights that covers what they and a score s + G are off by: 2^-24 of the scaled logits, several times over.
     __device__ __forceinline__ float spare() const { return 1.001f + fabsf(m) * 1e-6f; }
 };
@@ -247,8 +254,9 @@ __global__ void __launch_bounds__(VD_THREADS, DRAWS ? 4 : 5) parts_kernel(VdArgs
     float most = -INFINITY;
 #pragma unroll
     for (int k = 0; k < VD_GROUPS; ++k) most = fmaxf(most, fmaxf(fmaxf(v[k][0], v[k][1]), fmaxf(v[k][2], v[k][3])));
-    const float temp = a.temperature[r], m = warp_max(most) / temp;
-    const Weights weight(temp, m);
+    const float temp = a.temperature[r], largest = warp_max(most);
+    Weights weight(temp, largest);
+    const float m = weight.m;
     float z = 0.f;
     if (weight.odd) {
         if (m > -INFINITY) {
@@ -259,12 +267,21 @@ __global__ void __launch_bounds__(VD_THREADS, DRAWS ? 4 : 5) parts_kernel(VdArgs
             }
         }
     } else {                                                 // from here on v is the weight
+        if (!weight.near()) {                                // distances from the largest, which is 0 then
+#pragma unroll
+            for (int k = 0; k < VD_GROUPS; ++k)
+#pragma unroll
+                for (int q = 0; q < 4; ++q) v[k][q] -= largest;
+            most -= largest;
+            weight.most = weight.m2 = 0.f;
+        }
 #pragma unroll
         for (int k = 0; k < VD_GROUPS; ++k) {
 #pragma unroll
             for (int q = 0; q < 4; ++q) v[k][q] = weight.fast(v[k][q]);
             z += (v[k][0] + v[k][1]) + (v[k][2] + v[k][3]);
         }
+        z *= ex2(-weight.lost());
         most = weight.fast(most);
     }
     z = warp_sum(z);
@@ -321,7 +338,7 @@ __global__ void __launch_bounds__(VD_THREADS, DRAWS ? 4 : 5) parts_kernel(VdArgs
         }
         b = warp_best(b);
     }
-    if (lane == 0) *part = Part{m, z, b.v, b.i};
+    if (lane == 0) *part = Part{largest, z, b.v, b.i};
 }
 
 // What a warp's parts of a row come to: all of it for the row's warp.
@@ -333,6 +350,7 @@ __device__ __forceinline__ RowStats whole_row(const VdArgs& a, const Place& at, 
     const float at_draft = !greedy && drafted >= 0 && drafted < a.vocab ? at.x[drafted] : NAN;
     Best b{0.f, -1};
     float z = 0.f;
+    const float c = LOG2E / temp;
     for (int first = lane; first < n; first += 5 * 32) {     // five loads in flight
         Part p[5];
 #pragma unroll
@@ -341,17 +359,26 @@ __device__ __forceinline__ RowStats whole_row(const VdArgs& a, const Place& at, 
         for (int k = 0; k < 5; ++k) {
             b = better(b, Best{p[k].v, p[k].i});
             if (!greedy && p[k].z > 0.f) {
-                if (p[k].m > st.m) { z *= scaled_weight(st.m, p[k].m); st.m = p[k].m; }
-                z += p[k].z * scaled_weight(p[k].m, st.m);
+                if (p[k].m > st.m) { z *= ex2((st.m - p[k].m) * c); st.m = p[k].m; }
+                z += p[k].z * ex2((p[k].m - st.m) * c);
             }
         }
     }
     st.drawn = warp_best(b).i;
     if (greedy) return st;
-    const float m = warp_max(st.m);
-    st.z = warp_sum(z > 0.f ? z * scaled_weight(st.m, m) : 0.f);
-    st.m = m;
-    if (at_draft > -INFINITY) st.share = Weights(temp, m)(at_draft) / st.z;
+    const Weights weight(temp, warp_max(st.m));
+    if (weight.odd) {                                        // once more, by the quotients
+        z = 0.f;
+        for (int i = lane; i < n; i += 32) {
+            const Part p = nth(i);
+            if (p.z > 0.f) z += p.z * weight.quotient(p.m);
+        }
+    } else if (z > 0.f) {
+        z *= ex2((st.m - weight.most) * c);
+    }
+    st.z = warp_sum(z);
+    st.m = weight.most;
+    if (at_draft > -INFINITY) st.share = weight(at_draft) / st.z;
     return st;
 }
 
@@ -497,6 +524,7 @@ __global__ void __launch_bounds__(VD_THREADS, 4) rows_kernel(VdArgs a) {
     const float at_draft = drafted >= 0 && drafted < a.vocab ? at.x[drafted] : NAN;
     const bool lists = !at.draws && (int)blockIdx.x <= D;    // a draw behind a failed draft may want them
     RowStats st{0.f, 0.f, 0u, -1, 0.f, -1, {0, 0}};
+    float m = 0.f;                                           // the largest, scaled
     unsigned long long sum = 0;                              // weights of at most 1 in steps of 2^-44
     Best b{0.f, -1};
     asm volatile("cp.async.wait_all;" ::: "memory");
@@ -574,7 +602,7 @@ __global__ void __launch_bounds__(VD_THREADS, 4) rows_kernel(VdArgs a) {
     const int n = fits ? sh.count : a.vocab;
     auto take = [&](float s, int token) {
         if (score_key(s) < st.threshold) return;
-        sum += __float2ull_rn(scaled_weight(s, st.m) * 17592186044416.f);
+        sum += __float2ull_rn(scaled_weight(s, m) * 17592186044416.f);
         if (at.draws) b = better(b, Best{s - logf(exponential_of(token, c1, stream, 0u, key2)), token});
         if (lists && fits) {
             const int to = atomicAdd(&sh.listed, 1);
@@ -586,7 +614,7 @@ __global__ void __launch_bounds__(VD_THREADS, 4) rows_kernel(VdArgs a) {
         const unsigned first = tid < n ? sh.key[tid] : 0u, second = tid + VD_THREADS < n ? sh.key[tid + VD_THREADS] : 0u;
         const Range found = key_range(first, second, sh.range);
         if (n >= topk) st.threshold = n == topk ? found.least : reached_by(first, second, n > VD_THREADS, found.least, found.most, topk, 0);
-        st.m = n > 0 ? key_value(found.most) : -INFINITY;
+        m = n > 0 ? key_value(found.most) : -INFINITY;
     } else {
         // many candidates; or more than there is room for (a k in the thousands, thousands of equal logits): the row itself
         auto each = [&](auto f) {                            // every candidate's scaled logit
@@ -597,7 +625,7 @@ __global__ void __launch_bounds__(VD_THREADS, 4) rows_kernel(VdArgs a) {
             }
         };
         if (n >= topk) st.threshold = select_kth(topk, sh.hist, sh.sel, [&](auto count) { each([&](float s, int) { count(score_key(s)); }); });
-        st.m = most / temp;                                  // (quotients keep the order of what is divided)
+        m = most / temp;                                     // (quotients keep the order of what is divided)
         if (!fits) {
             each([&](float s, int token) { take(s, token); });
             if (tid == 0) sh.listed = a.list + 1;
@@ -621,9 +649,10 @@ __global__ void __launch_bounds__(VD_THREADS, 4) rows_kernel(VdArgs a) {
     }
     if (lane > 0) return;
     st.z = (float)((double)sum * (1.0 / 17592186044416.0));
+    st.m = most;
     st.drawn = b.i;
     const float s = at_draft / temp;
-    if (s > -INFINITY && score_key(s) >= st.threshold) st.share = scaled_weight(s, st.m) / st.z;
+    if (s > -INFINITY && score_key(s) >= st.threshold) st.share = scaled_weight(s, m) / st.z;
     if (lists && sh.listed <= a.list) st.listed = sh.listed;
     a.stats[slot] = st;
 }
@@ -705,7 +734,7 @@ __global__ void __launch_bounds__(VD_THREADS, JUDGED ? 4 : 1) verify_kernel(VdAr
                 // (second: nothing of p lies beyond q, they differ by a rounding: p itself)
 #pragma unroll 1
                 for (float q_share = 1.f; q_share >= 0.f && b.i < 0; q_share -= 1.f) {
-                    for (int i = tid; i < st.listed; i += VD_THREADS) race(scaled_weight(list[i].s, st.m) * pz - q_share * q_of(y[list[i].i]), list[i].i);
+                    for (int i = tid; i < st.listed; i += VD_THREADS) race(scaled_weight(list[i].s, pw.m) * pz - q_share * q_of(y[list[i].i]), list[i].i);
                     b = block_best(b, best_sh);
                 }
             } else {
@@ -726,15 +755,18 @@ __global__ void __launch_bounds__(VD_THREADS, JUDGED ? 4 : 1) verify_kernel(VdAr
                     }
                     asm volatile("cp.async.commit_group;" ::: "memory");
                 };
-                // Logits that no threshold and no infinity cuts: a share is 2^(v c - m log2 e - log2 z). Otherwise by p_of and q_of.
-                const bool plain = !st.threshold && !ds.threshold && !pw.odd && !(failed && qw.odd) && st.z > 0.f;
-                const float p2 = pw.m2 + log2f(st.z), q2 = failed ? qw.m2 + log2f(ds.z) : INFINITY;
+                // Logits that no threshold and no infinity cuts: a share is 2^(v c - most c - log2 z). Otherwise by p_of and q_of.
+                // What rounding takes from the constants makes a factor, of p's share against q's.
+                const bool plain = !st.threshold && !ds.threshold && pw.near() && !pw.odd && (!failed || (qw.near() && !qw.odd)) && st.z > 0.f;
+                const float pl = log2f(st.z), p2 = pw.m2 + pl, ql = log2f(ds.z), q2 = failed ? qw.m2 + ql : INFINITY;
+                auto rest = [](float a, float b, float sum) { return fabsf(a) < fabsf(b) ? (b - sum) + a : (a - sum) + b; };
+                const float q_factor = failed ? ex2(rest(pw.m2, pl, p2) + pw.lost() - (rest(qw.m2, ql, q2) + qw.lost())) : 0.f;
                 // Only tokens whose share can still pass the best B of the block run: share / E > B needs 1 - U < share / B.
                 unsigned beaten = 0u;                        // B as a key, as this warp knows it
                 float spare = INFINITY;                      // 1 / B, with something to spare
                 auto beat = [&](unsigned key) {
                     beaten = key;
-                    spare = pw.spare() * (failed ? 1.f / key_value(key) : ex2((st.m - key_value(key)) * LOG2E) * st.z);
+                    spare = pw.spare() * (failed ? 1.f / key_value(key) : ex2((pw.m - key_value(key)) * LOG2E) * st.z);
                 };
 #pragma unroll 1
                 for (int k = 0; k < VD_STAGES; ++k) fetch(slot + k * STAGE, (rank + k * ctas) * VD_THREADS + tid);
@@ -748,7 +780,10 @@ __global__ void __launch_bounds__(VD_THREADS, JUDGED ? 4 : 1) verify_kernel(VdAr
                     float p[4];
                     if (plain) {
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) p[i] = ex2(fmaf(fmaxf(v[i], -INFINITY), pw.c, -p2)) - ex2(fmaf(fmaxf(q[i], -INFINITY), pw.c, -q2));
+                        for (int i = 0; i < 4; ++i) {
+                            const float beyond = ex2(fmaf(fmaxf(q[i], -INFINITY), pw.c, -q2));
+                            p[i] = fmaf(-q_factor, beyond, ex2(fmaf(fmaxf(v[i], -INFINITY), pw.c, -p2)));
+                        }
                     } else {
 #pragma unroll
                         for (int i = 0; i < 4; ++i) p[i] = p_of(v[i]) - (failed ? q_of(q[i]) : 0.f);
