@@ -169,3 +169,28 @@ def test_temperatures_near_0(ops, shift, topk):
     assert check(ops, x, fed, opts) >= s // 3
     for q in (x[:, :1], x[:, :1] + 0.5 * torch.randn(s, 1, vocab, generator=g).to(dev())):
         check(ops, x, fed, opts, q)
+
+
+@pytest.mark.parametrize("vocab", [600, 40007])
+@pytest.mark.parametrize("topk", [0, 7, 300])
+def test_rows_whose_quotients_are_all_infinite(ops, vocab, topk):
+    """The type's lowest value over a temperature below 1 is -inf: such a row has nothing, as one of -inf has. No draft holds, not the
+    first finite logit's either, and the token is the one that sample gives. At a temperature of 1 or more all tokens are alike."""
+    temperature = [0.3, 0.5, 0.7, 0.99, 1.0, 1.3]
+    s = len(temperature)
+    x = torch.full((s, 2, vocab), torch.finfo(torch.float32).min, device=dev())
+    x[:, :, :5] = float("-inf")
+    opts = options(temperature, [topk] * s, seed=21)
+    other = torch.randn(s, 1, vocab, generator=torch.Generator().manual_seed(4)).to(dev())
+    first = ops.sample(x[:, 0].contiguous(), *(opts[n] for n in NAMES)).tolist()
+    for draft in (5, 6, 0, vocab - 1):
+        fed = [[1, draft]] * s
+        for q in (None, other, x[:, :1]):
+            check(ops, x, fed, opts, q)
+            got = ops.verify_drafts(x.reshape(2 * s, vocab), ints(fed).flatten(), ints(range(0, 2 * s + 1, 2)), max_drafts=1,
+                                    draft_logits=q, **opts)
+            assert got.tokens[:4].tolist() == [[0, -1]] * 4 and got.counts[:4].tolist() == [1] * 4 and not got.accept[:4].any()
+            if q is None:
+                assert got.tokens[:, 0].tolist() == first
+    # the target has something, the draft model's row nothing: what p gives anything holds
+    check(ops, other.expand(s, 2, vocab).contiguous(), [[1, int(other[r, 0].argmax())] for r in range(s)], opts, x[:, :1])

@@ -327,7 +327,8 @@ __global__ void __launch_bounds__(VD_THREADS, DRAWS ? 4 : 5) parts_kernel(VdArgs
             for (; left; left &= left - 1u) {                // (their numbers once more: the register file has no subscripts)
                 const int bit = __ffs(left) - 1, i = token_of(blockIdx.x, tid, bit >> 2) + (bit & 3);
                 const uint4 w = philox4x32_10(make_uint4((unsigned)i >> 2, c1, stream, 0u), key2);
-                b = better(b, Best{noisy(at.x[i] / temp, philox_uniform(word_of(w, i))), i});
+                const float s = at.x[i] / temp;              // (-inf, too, of a finite logit at a temperature below 1)
+                if (s > -INFINITY) b = better(b, Best{noisy(s, philox_uniform(word_of(w, i))), i});
             }
             if (half == 0) {                                 // the best that any warp of the block has found
                 const float own = warp_max(b.i < 0 ? -INFINITY : b.v);
@@ -378,7 +379,7 @@ __device__ __forceinline__ RowStats whole_row(const VdArgs& a, const Place& at, 
     }
     st.z = warp_sum(z);
     st.m = weight.most;
-    if (at_draft > -INFINITY) st.share = weight(at_draft) / st.z;
+    if (at_draft > -INFINITY && st.z > 0.f) st.share = weight(at_draft) / st.z;
     return st;
 }
 
@@ -601,7 +602,7 @@ __global__ void __launch_bounds__(VD_THREADS, 4) rows_kernel(VdArgs a) {
     Kept* kept = lists ? a.kept + ((size_t)r * D + at.j) * a.list : nullptr;
     const int n = fits ? sh.count : a.vocab;
     auto take = [&](float s, int token) {
-        if (score_key(s) < st.threshold) return;
+        if (score_key(s) < st.threshold || !(s > -INFINITY)) return;
         sum += __float2ull_rn(scaled_weight(s, m) * 17592186044416.f);
         if (at.draws) b = better(b, Best{s - logf(exponential_of(token, c1, stream, 0u, key2)), token});
         if (lists && fits) {
