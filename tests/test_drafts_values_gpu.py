@@ -194,3 +194,31 @@ def test_rows_whose_quotients_are_all_infinite(ops, vocab, topk):
                 assert got.tokens[:, 0].tolist() == first
     # the target has something, the draft model's row nothing: what p gives anything holds
     check(ops, other.expand(s, 2, vocab).contiguous(), [[1, int(other[r, 0].argmax())] for r in range(s)], opts, x[:, :1])
+
+
+@pytest.mark.parametrize("scale", [1e-4, 1.0, 1e6])
+@pytest.mark.parametrize("topk", [0, 50])
+def test_quotients_that_rounding_makes_equal(ops, scale, topk):
+    """Logits a step of float32 apart over temperatures near 0: their quotients differ by less than a rounding, so some are equal, the
+    noise of others is lost beside them, and of equal scores the first wins. The token is the one that sample gives, drafts of it hold,
+    also behind drafts that are sure to hold against the same draft logits."""
+    vocab, temperature = 5003, [10.0 ** -e for e in range(3, 28)] * 2
+    s = len(temperature)
+    g = torch.Generator().manual_seed(31)
+    top = (20.0 + 4.0 * torch.rand(s, 2, 1, generator=g)) * scale * torch.where(torch.rand(s, 2, 1, generator=g) < 0.3, -1.0, 1.0)
+    steps = torch.randint(0, 9, (s, 2, vocab), generator=g, dtype=torch.int32)
+    x = (top.view(torch.int32) - steps * torch.sign(top).int()).view(torch.float32)
+    x[:, :, ::3] -= 5.0 * scale
+    x = x.to(dev())
+    opts = options(temperature, [topk] * s, seed=32)
+    rows = [x[:, j].contiguous() for j in range(2)]
+    first = ops.sample(rows[0], *(opts[n] for n in NAMES))
+    second = ops.sample(rows[1], *(opts["step"] + 1 if n == "step" else opts[n] for n in NAMES))
+    fed = torch.stack((first, first), 1).flatten()
+    cu = ints(range(0, 2 * s + 1, 2))
+    got = ops.verify_drafts(x.reshape(2 * s, vocab), fed, cu, max_drafts=1, **opts)
+    assert got.tokens[:, 0].tolist() == first.tolist() and got.counts.tolist() == [2] * s
+    assert got.tokens[:, 1].tolist() == second.tolist()
+    sure = ops.argmax(rows[0])                           # p = q there: it holds
+    got = ops.verify_drafts(x.reshape(2 * s, vocab), torch.stack((sure, sure), 1).flatten(), cu, max_drafts=1, draft_logits=x[:, :1], **opts)
+    assert got.counts.tolist() == [2] * s and got.tokens[:, 1].tolist() == second.tolist()

@@ -124,9 +124,13 @@ struct Weights {
         return !(s > -INFINITY) ? 0.f : (s == m ? 1.f : expf(s - m));
     }
     __device__ __forceinline__ float operator()(float v) const { return odd ? quotient(v) : ex2((v - most) * c); }
-    // A factor on the weights that covers what they and a score s + G are off by: 2^-24 of the scaled logits, several times over.
+    // A factor on the weights that covers what they and a score s + G are off by, near 0: `lost`, 2^-24 of the scaled logits each for
+    // two quotients and two sums, some steps of the functions; together below e^(4e-7 |m|) + 1e-4. (Farther off the quotients' own
+    // roundings decide: equal ones are a tie, whatever their logits.)
     __device__ __forceinline__ float spare() const { return 1.001f + fabsf(m) * 1e-6f; }
 };
+// Whether s + G may reach a score: G is 16.7 at most, and the sum is rounded.
+__device__ __forceinline__ bool may_reach(float s, float score) { return s > -INFINITY && s + fmaf(fabsf(s), 2.4e-7f, 17.f) >= score; }
 // The same of a scaled logit at hand.
 __device__ __forceinline__ float scaled_weight(float s, float m) { return !(s > -INFINITY) ? 0.f : (s == m ? 1.f : ex2((s - m) * LOG2E)); }
 
@@ -291,7 +295,7 @@ __global__ void __launch_bounds__(VD_THREADS, DRAWS ? 4 : 5) parts_kernel(VdArgs
         // is exact: one comparison settles all but a few tokens once some B is known.
         const uint2 key2 = seed_of(a, r);
         const unsigned c1 = (unsigned)a.step[r] + (unsigned)at.j, stream = (unsigned)a.stream_id[r];
-        float spare = 0.f;                                   // exp(m - B)
+        float spare = 0.f, score = -INFINITY;                // exp(m - B), B
 #pragma unroll 1
         for (int half = 0; half < 2; ++half) {               // the threads' largest logits for a first B, then all
             unsigned left = 0u;
@@ -300,6 +304,12 @@ __global__ void __launch_bounds__(VD_THREADS, DRAWS ? 4 : 5) parts_kernel(VdArgs
                 for (int k = 0; k < VD_GROUPS; ++k)
 #pragma unroll
                     for (int q = 0; q < 4; ++q) left = v[k][q] == most ? 1u << (4 * k + q) : left;
+            } else if (weight.odd || !weight.near()) {       // by the quotients
+#pragma unroll 1
+                for (int i = 0; i < 4 * VD_GROUPS; ++i) {
+                    const int e = token_of(blockIdx.x, tid, i >> 2) + (i & 3);
+                    if (e < a.vocab && may_reach(at.x[e] / temp, score)) left |= 1u << i;
+                }
             } else {
                 // round by round for all groups: they share the key's bumps and what the first rounds make of the step and the stream
                 // (320 open rows of 151,936 looked-up drafts 94 us; group by group 104)
@@ -320,7 +330,7 @@ __global__ void __launch_bounds__(VD_THREADS, DRAWS ? 4 : 5) parts_kernel(VdArgs
                     const unsigned words[4] = {w[k].x, w[k].y, w[k].z, w[k].w};
 #pragma unroll
                     for (int q = 0; q < 4; ++q)
-                        left |= (weight.odd ? v[k][q] > -INFINITY : may_pass(words[q], v[k][q], spare)) ? 1u << (4 * k + q) : 0u;
+                        left |= may_pass(words[q], v[k][q], spare) ? 1u << (4 * k + q) : 0u;
                 }
             }
             if (half == 0 && !(most > (weight.odd ? -INFINITY : 0.f))) left = 0u;       // (a weight of nothing is beaten by the largest)
@@ -334,7 +344,8 @@ __global__ void __launch_bounds__(VD_THREADS, DRAWS ? 4 : 5) parts_kernel(VdArgs
                 const float own = warp_max(b.i < 0 ? -INFINITY : b.v);
                 if (lane == 0) best_sh[tid >> 5] = own;
                 __syncthreads();
-                spare = ex2((m - warp_max(best_sh[lane & (VD_WARPS - 1)])) * LOG2E) * weight.spare();
+                score = warp_max(best_sh[lane & (VD_WARPS - 1)]);
+                spare = ex2((m - score) * LOG2E) * weight.spare();
             }
         }
         b = warp_best(b);
@@ -546,7 +557,7 @@ __global__ void __launch_bounds__(VD_THREADS, 4) rows_kernel(VdArgs a) {
                                                       : lines_reached_by(sh, largest, n_lines, offered.most, topk, topk / 8);
     // (What lies 110 below the largest, scaled, has no weight in float32 and no noise that makes up for it: the tokens that a mask of the
     // type's lowest value leaves behind its own are not candidates, though the threshold may not drop them.)
-    const float most = key_value(offered.most), floor = fabsf(most / temp) < 1e30f ? most - 110.f * temp : -INFINITY;
+    const float most = key_value(offered.most), floor = fabsf(most / temp) < 1e30f ? most - 110.f * temp - fabsf(most) * 4.8e-7f : -INFINITY;
     const float low = fmaxf(below_quotient(key_value(bound), temp), floor);
     constexpr int FOURS = 5;                                 // groups of four a thread looks at together
 #pragma unroll 1
@@ -720,7 +731,9 @@ __global__ void __launch_bounds__(VD_THREADS, JUDGED ? 4 : 1) verify_kernel(VdAr
             const RowStats ds = failed ? row_sh[D + 1 + held] : RowStats{0.f, 0.f, 0u, -1, 0.f, -1, {0, 0}};
             const float* x = a.logits + (size_t)(rows.x + held) * a.vocab;
             const float* y = failed ? a.draft_logits + r * a.draft_request + held * a.draft_place : x;
-            const Weights pw(temp, st.m), qw(temp, ds.m);
+            Weights pw(temp, st.m);
+            const Weights qw(temp, ds.m);
+            pw.odd |= !failed && !pw.near();                 // a draw from p alone goes by the quotients
             const float pz = st.z > 0.f ? 1.f / st.z : 0.f, qz = ds.z > 0.f ? 1.f / ds.z : 0.f;
             auto p_of = [&](float v) { return v > -INFINITY && (!st.threshold || score_key(v / temp) >= st.threshold) ? pw(v) * pz : 0.f; };
             auto q_of = [&](float v) { return v > -INFINITY && (!ds.threshold || score_key(v / temp) >= ds.threshold) ? qw(v) * qz : 0.f; };
