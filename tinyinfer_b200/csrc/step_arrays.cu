@@ -111,7 +111,9 @@ TI_API int ti_step_arrays(int* token_ids, int* positions, int* token_seq, int* c
     TI_REQUIRE(requests >= 0 && requests < 65535 && groups >= 1 && table_rows >= 0 && width >= 1 && rows >= 0 && max_count >= 1 && page_size >= 1,
                "step_arrays: bad sizes");
     TI_REQUIRE(rows < (1 << 30) && max_count < (1 << 30), "step_arrays: fewer than 2^30 rows");     // two of them add up to less than 2^31
-    TI_REQUIRE((token_ids == nullptr) == (tokens == nullptr) && (!tokens || token_width >= max_count), "step_arrays: tokens narrower than max_count");
+    // (an array without entries may have no address: without requests nothing is read from tokens, without rows nothing is written)
+    TI_REQUIRE(requests == 0 || rows == 0 || (token_ids == nullptr) == (tokens == nullptr), "step_arrays: token_ids and tokens go together");
+    TI_REQUIRE(!tokens || token_width >= max_count, "step_arrays: tokens narrower than max_count");
     SaArgs a{starts, counts, state_slots, tables, tokens, token_ids, positions, token_seq, cache_slots, cu_seqlens, q_starts, context_lens,
              (int4*)tiles, block_tables, status, requests, groups, table_rows, width, token_width, rows, max_count,
              (max_count + SA_TILE - 1) / SA_TILE, page_size, pad_page};
