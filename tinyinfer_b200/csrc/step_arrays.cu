@@ -2,6 +2,7 @@
 // and brings counts[s]. Flat row cu[s] + i (cu: the sums of the counts before) is its token at position starts[s] + i, whose key goes to
 // slot page * page_size + position % page_size of the page that the request's block table has for it. Rows behind the last
 // request are position 0 of a request of their own (number `requests`) whose only page is pad_page.
+// What is left out sets the status word, which keeps the larger of two codes: it does not depend on which block comes last.
 // Pure data movement: every block adds up the counts before its request itself (they lie in L2), so one launch does it all.
 #include "common.cuh"
 
@@ -69,7 +70,7 @@ __global__ void __launch_bounds__(SA_THREADS) step_arrays_kernel(SaArgs a) {
             if (pad) a.cu_seqlens[s + 1] = a.rows;
             a.q_starts[s] = start;
             a.context_lens[s] = context;
-            if (cut && a.status) atomicExch(a.status, 5);
+            if (cut && a.status) atomicMax(a.status, 5);
         }
         if (!pad)
             for (int i = tid; i < a.tiles_each; i += SA_THREADS) {
@@ -97,7 +98,7 @@ __global__ void __launch_bounds__(SA_THREADS) step_arrays_kernel(SaArgs a) {
             const long long at = (long long)page * a.page_size + pos % a.page_size;
             const bool ok = page >= 0 && at <= 0x7FFFFFFFll;
             a.cache_slots[(size_t)g * a.rows + row] = ok ? (int)at : -1;
-            if (!ok && !pad && a.status) atomicExch(a.status, 1);     // a token without a page
+            if (!ok && !pad && a.status) atomicMax(a.status, 1);      // a token without a page
         }
     }
 }

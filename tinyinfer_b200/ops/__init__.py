@@ -2580,7 +2580,7 @@ def step_arrays(starts: torch.Tensor, counts: torch.Tensor, block_tables: torch.
     kernels take them. ``block_tables``: the pages up to each request's end, -1 behind them, number S's last.
 
     What does not fit into ``max_count`` or ``rows``, and a request whose row or start does not exist, is left out and sets the
-    ``status`` word, as a token without a page does (``page_status``)."""
+    ``status`` word, as a token without a page does (``page_status``). Where both happen the word tells of what was left out."""
     rows, max_count, page_size, pad_page = int(rows), int(max_count), int(page_size), int(pad_page)
     _check(starts, "starts", torch.int32, 1)
     s, device = starts.shape[0], starts.device
