@@ -4,8 +4,10 @@
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
+#include <atomic>
 #include <cstdint>
 #include <cstdio>
+#include <mutex>
 
 #define TI_API extern "C" __attribute__((visibility("default")))
 
@@ -72,17 +74,21 @@ cudaError_t ti_launch_alone(void (*kernel)(KArgs...), dim3 grid, dim3 block, siz
 }
 
 // Lets KERNEL have `bytes` of dynamic shared memory on the current device. The attribute belongs to a device, and so does the
-// record of having set it (beyond 64 devices it is set on every call).
+// record of having set it (beyond 64 devices it is set on every call). Threads that ask for different sizes at once take turns: what
+// one was allowed is not lowered behind it.
 template <auto KERNEL>
 cudaError_t ti_allow_shared(int bytes) {
     constexpr int DEVICES = 64;
-    static int allowed[DEVICES] = {};
+    static std::atomic<int> allowed[DEVICES];
+    static std::mutex turn;
     int dev = -1;
     const cudaError_t got = cudaGetDevice(&dev);
     if (got != cudaSuccess) return got;
-    if (dev < DEVICES && allowed[dev] >= bytes) return cudaSuccess;
+    if (dev < DEVICES && allowed[dev].load() >= bytes) return cudaSuccess;
+    std::lock_guard<std::mutex> hold(turn);
+    if (dev < DEVICES && allowed[dev].load() >= bytes) return cudaSuccess;
     const cudaError_t e = cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-    if (e == cudaSuccess && dev < DEVICES) allowed[dev] = bytes;
+    if (e == cudaSuccess && dev < DEVICES) allowed[dev].store(bytes);
     return e;
 }
 
