@@ -41,3 +41,37 @@ def test_the_status_word_keeps_what_was_left_out(ops, starts, counts):
         word = torch.zeros(1, dtype=torch.int32, device=dev())
         ops.step_arrays(ints(starts), ints(counts), table, rows=20, max_count=4, page_size=8, status=word)
         assert word.item() == 5
+
+
+def test_the_loop_that_the_readme_shows(ops):
+    """Its lines, run as they stand around a model whose logits are a function of a token and its position: the texts are those of
+    decoding one by one."""
+    import re
+    from pathlib import Path
+    readme = (Path(__file__).resolve().parent.parent / "README.md").read_text()
+    lines = next(b for b in re.findall(r"```python\n(.*?)```", readme, re.S) if "ngram_drafts" in b)
+    S, D, vocab, longest, steps = 4, 3, 29, 200, 25
+    g = torch.Generator().manual_seed(2)
+    table = (3.0 * torch.randn(vocab, 2, vocab, generator=g)).to(dev())
+    prompts, sampling = ints([3, 9, 1, 6]), dict(
+        temperature=torch.tensor([1.0, 0.8, 0.5, 1.2], device=dev()), topk=ints([0, 5, 0, 0]), greedy=ints([1, 0, 0, 0]),
+        seed=ints([1, 2, 3, 4], torch.int64), stream_id=ints([5, 6, 7, 8]))
+    history = torch.randint(0, vocab, (S, longest), generator=g, dtype=torch.int32).to(dev())
+    first, n = history.clone(), prompts.tolist()
+    names = dict(S=S, D=D, history=history, lengths=prompts.clone(), prompts=prompts, spare_page=99, **sampling,
+                 block_tables=torch.arange(S * 4, dtype=torch.int32, device=dev()).view(S, 4),
+                 model=lambda step: table[step.token_ids.long(), step.positions.long() % 2].contiguous(),
+                 found=ops.VerifiedDrafts(torch.full((S, D + 1), -1, dtype=torch.int32, device=dev()), ints([0] * S), None))
+    held = 0
+    for _ in range(steps):
+        exec(lines, names)
+        held += int((names["found"].counts - 1).sum())
+    assert held > 5
+    for r in range(S):
+        text, made = first[r, :n[r]].tolist(), int(names["lengths"][r]) - n[r]
+        assert made >= steps - 1
+        for i in range(made):
+            row = table[text[-1], (len(text) - 1) % 2][None].contiguous()
+            one = {k: t[r:r + 1].contiguous() for k, t in sampling.items()}
+            text.append(int(ops.sample(row, one["temperature"], one["topk"], one["greedy"], one["seed"], one["stream_id"], ints([i]))))
+        assert history[r, :len(text)].tolist() == text, r
