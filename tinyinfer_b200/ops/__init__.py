@@ -12,6 +12,7 @@ from __future__ import annotations
 
 import array
 import ctypes
+import functools
 from typing import NamedTuple, Optional, Sequence
 
 import torch
@@ -2456,6 +2457,8 @@ def verify_drafts(logits: torch.Tensor, token_ids: torch.Tensor, cu_rows: torch.
     drafts and that draw behind one that failed against ``draft_logits`` are apart from the noise of ``sample``, which the drafts may
     have been drawn with.
 
+    The result's tensors share one allocation, with up to 1 MB that the call worked in: who keeps one of them for long keeps a copy of it.
+
     A draft outside the vocabulary never holds. NaN logits are passed over, as ``sample`` does; a sampled row with nothing but NaN and
     -inf lets no draft hold and gives token 0."""
     _check(logits, "logits", torch.float32, 2)
@@ -2505,14 +2508,12 @@ def verify_drafts(logits: torch.Tensor, token_ids: torch.Tensor, cu_rows: torch.
     return VerifiedDrafts(tokens, counts, accept)
 
 
+@functools.lru_cache(maxsize=4096)
 def _verify_scratch_words(*key) -> int:
     """(requests, max_drafts, vocab, sampled, with draft logits) -> 32-bit words."""
-    n = _scratch_floats.get(("verify", *key))
-    if n is None:
-        fn = _fn("drafts", "ti_verify_scratch_words")
-        fn.restype = ctypes.c_longlong
-        n = _scratch_floats["verify", *key] = int(fn(*key))
-    return n
+    fn = _fn("drafts", "ti_verify_scratch_words")
+    fn.restype = ctypes.c_longlong
+    return int(fn(*key))
 
 
 def ngram_drafts(history: torch.Tensor, lengths: torch.Tensor, *, max_drafts: int, max_match: int = 3, min_match: int = 1,
