@@ -222,3 +222,20 @@ def test_quotients_that_rounding_makes_equal(ops, scale, topk):
     sure = ops.argmax(rows[0])                           # p = q there: it holds
     got = ops.verify_drafts(x.reshape(2 * s, vocab), torch.stack((sure, sure), 1).flatten(), cu, max_drafts=1, draft_logits=x[:, :1], **opts)
     assert got.counts.tolist() == [2] * s and got.tokens[:, 1].tolist() == second.tolist()
+
+
+@pytest.mark.parametrize("topk", [0, 20])
+@pytest.mark.parametrize("temperature", [1e30, 3e38, math.inf])
+def test_temperatures_that_make_all_tokens_alike(ops, temperature, topk):
+    vocab, s = 9001, 6
+    g = torch.Generator().manual_seed(41)
+    x = torch.randn(s, 2, vocab, generator=g).to(dev())
+    opts = options([temperature] * s, [topk] * s, seed=42)
+    drawn = ops.sample(x[:, 0].contiguous(), *(opts[n] for n in NAMES)).tolist()
+    fed = [[1, drawn[r] if r % 2 else (drawn[r] + 1) % vocab] for r in range(s)]
+    for q in (None, x[:, 1:], 30.0 * x[:, 1:]):
+        check(ops, x, fed, opts, q)
+    if topk and temperature == math.inf:                 # quotients of 0 and -0: equal here, as s >= k-th largest has it, not in sample
+        return
+    got = ops.verify_drafts(x.view(2 * s, vocab), ints(fed).flatten(), ints(range(0, 2 * s + 1, 2)), max_drafts=1, **opts)
+    assert got.tokens[:, 0].tolist() == drawn and got.counts.tolist() == [1 + r % 2 for r in range(s)]

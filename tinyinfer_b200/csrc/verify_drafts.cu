@@ -106,7 +106,7 @@ __device__ __forceinline__ float ex2(float x) {
 }
 // The weights of a row's logits by their distance from the largest, `most`: exp((v - most) / temp), which is 1 at the largest however far
 // the logits lie from 0 (a mask's -1e10, a temperature near 0): an error in (v - most) c is one of the distance alone. Where a quotient
-// is infinite, or the temperature's reciprocal nearly, the quotients themselves are compared.
+// is infinite, or the temperature's reciprocal 0 or nearly infinite, the quotients themselves are compared.
 // `fast`, for many logits at once, is one multiply-add and one exponential, 2^(v c - m2) with m2 = most c rounded: that is 2^lost off,
 // alike for all, and lost is an exact float32. At |m| < 2^20 (`near`) it is 0.09 at most; beyond, it may be anything (2^440 at -1e10).
 constexpr float NEAR = 1048576.f;
@@ -114,7 +114,7 @@ struct Weights {
     float temp, most, m, c, m2;
     bool odd;
     __device__ __forceinline__ Weights(float temp_, float most_) : temp(temp_), most(most_), m(most_ / temp_), c(LOG2E / temp_), m2(most_ * c) {
-        odd = !(fabsf(m) < INFINITY) || !(c < 1e30f);
+        odd = !(fabsf(m) < INFINITY) || !(c > 0.f && c < 1e30f);
     }
     __device__ __forceinline__ bool near() const { return fabsf(m) < NEAR; }
     __device__ __forceinline__ float lost() const { return fmaf(most, c, -m2); }
