@@ -75,3 +75,58 @@ def test_the_loop_that_the_readme_shows(ops):
             one = {k: t[r:r + 1].contiguous() for k, t in sampling.items()}
             text.append(int(ops.sample(row, one["temperature"], one["topk"], one["greedy"], one["seed"], one["stream_id"], ints([i]))))
         assert history[r, :len(text)].tolist() == text, r
+
+
+@pytest.mark.parametrize("n", [70001, 9000])
+@pytest.mark.parametrize("max_match,min_match", [(32, 1), (32, 32), (3, 2)])
+def test_long_texts_of_one_token(ops, n, max_match, min_match):
+    """Every place matches: the latest is taken. Behind one other token, which the longest matches do not pass, and repeated in pairs."""
+    texts = torch.full((4, n + 3), 7, dtype=torch.int32)
+    texts[1, n - 20] = 8
+    texts[2, ::2] = 6
+    texts[3, n - 1] = 8
+    got = ops.ngram_drafts(texts.to(dev()), ints([n] * 4), max_drafts=5, max_match=max_match, min_match=min_match)
+    for i in range(4):
+        text = texts[i, :n].tolist()
+        tail, best = text[-200:], (0, 0)
+        # a match ends as far back as 200 tokens only if none of that length stands nearer: the texts repeat within 25 tokens, or never match
+        for e in range(1, n) if i == 3 else list(range(n - 100, n)) + list(range(1, 100)):
+            l = 0
+            while l < min(max_match, e) and text[e - 1 - l] == text[n - 1 - l]:
+                l += 1
+            best = max(best, (l, e)) if l >= min_match else best
+        want = list(text)
+        for t in range(5 if best[0] else 0):
+            want.append(want[best[1] + t])
+        assert got.tokens[i].tolist() == text[-1:] + want[n:] + [-1] * (5 - len(want) + n), i
+
+
+def test_two_threads_at_once(ops):
+    """Each with its own stream and vocabulary, the larger of which needs more shared memory than any kernel has without asking."""
+    import threading
+
+    def job(vocab, out, barrier):
+        g = torch.Generator().manual_seed(vocab)
+        rows = (2.0 * torch.randn(8, vocab, generator=g)).to(dev())
+        opts = dict(temperature=torch.full((4,), 0.8, device=dev()), topk=ints([100] * 4), greedy=ints([0] * 4), stream_id=ints([1, 2, 3, 4]),
+                    seed=ints([5] * 4, torch.int64), step=ints([0] * 4))
+        want = ops.sample(rows[::2].contiguous(), *(opts[n] for n in ("temperature", "topk", "greedy", "seed", "stream_id", "step")))
+        fed = torch.stack((want, want), 1).flatten()
+        torch.cuda.synchronize()
+        stream = torch.cuda.Stream()
+        try:
+            with torch.cuda.stream(stream):
+                barrier.wait(60)
+                got = [ops.verify_drafts(rows, fed, ints([0, 2, 4, 6, 8]), max_drafts=1, **opts) for _ in range(20)]
+            stream.synchronize()
+            out.append(all(g.counts.tolist() == [2] * 4 and torch.equal(g.tokens[:, 0], want) for g in got))
+        except Exception as e:                           # noqa: BLE001 (said by the test's own thread)
+            out.append(e)
+
+    out, barrier, lock = [], threading.Barrier(2), [40007, 400009]
+    threads = [threading.Thread(target=job, args=(v, out, barrier)) for v in lock]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert out == [True, True]
