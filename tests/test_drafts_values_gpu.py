@@ -239,3 +239,19 @@ def test_temperatures_that_make_all_tokens_alike(ops, temperature, topk):
         return
     got = ops.verify_drafts(x.view(2 * s, vocab), ints(fed).flatten(), ints(range(0, 2 * s + 1, 2)), max_drafts=1, **opts)
     assert got.tokens[:, 0].tolist() == drawn and got.counts.tolist() == [1 + r % 2 for r in range(s)]
+
+
+@pytest.mark.parametrize("vocab", [700, 30011])
+def test_zeros_of_either_sign_at_the_threshold(ops, vocab):
+    """s >= the k-th largest keeps -0 where that is +0: the draws and the shares are those of all zeros, many more than k."""
+    s, k = 8, 5
+    x = torch.full((s, 2, vocab), -1.0)
+    x[:, :, :200:2], x[:, :, 1:200:2] = 0.0, -0.0
+    x[:, :, 300] = 1.0
+    x = x.to(dev())
+    opts = options([0.5, 1.0] * 4, [k] * s, seed=51)
+    other = torch.randn(s, 1, vocab, generator=torch.Generator().manual_seed(52)).to(dev())
+    for draft in (0, 1, 300, 500):
+        for q in (None, other):
+            assert check(ops, x, [[1, draft]] * s, opts, q) >= s // 2
+        check(ops, x, [[1, draft]] * s, opts, x[:, 1:])  # (p = q: nothing is left beyond it, which float32 cannot tell from next to nothing)

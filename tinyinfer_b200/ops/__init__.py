@@ -2460,7 +2460,8 @@ def verify_drafts(logits: torch.Tensor, token_ids: torch.Tensor, cu_rows: torch.
     The result's tensors share one allocation, with up to 1 MB that the call worked in: who keeps one of them for long keeps a copy of it.
 
     A draft outside the vocabulary never holds. NaN logits are passed over, as ``sample`` does; a sampled row with nothing but NaN and
-    -inf lets no draft hold and gives token 0."""
+    -inf, or whose quotients by the temperature are all -inf, lets no draft hold and gives token 0. One thing differs from ``sample``: at the
+    top-k threshold -0 and +0 are one value here, so that both are kept, where ``sample`` takes -0 for the lower."""
     _check(logits, "logits", torch.float32, 2)
     _check(token_ids, "token_ids", torch.int32, 1)
     _check(cu_rows, "cu_rows", torch.int32, 1)
