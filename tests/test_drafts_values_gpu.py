@@ -255,3 +255,22 @@ def test_zeros_of_either_sign_at_the_threshold(ops, vocab):
         for q in (None, other):
             assert check(ops, x, [[1, draft]] * s, opts, q) >= s // 2
         check(ops, x, [[1, draft]] * s, opts, x[:, 1:])  # (p = q: nothing is left beyond it, which float32 cannot tell from next to nothing)
+
+
+@pytest.mark.parametrize("size", [1.04e6, 1.05e6, 5e7, 5.36e8, 5.38e8, 1.08e9, 3e12])
+def test_where_the_noise_fades(ops, size):
+    """Scaled logits from where a step of float32 is a sixteenth to where it is past all noise, of either sign, in two to nine neighbouring
+    values of float32, some tiles nothing but the lower ones: the tokens are sample's."""
+    vocab, s = 30011, 8
+    g = torch.Generator().manual_seed(61)
+    top = torch.tensor([-size, size] * (s // 2)).view(s, 1, 1).expand(s, 2, 1).contiguous()
+    steps = torch.randint(0, 9, (s, 2, vocab), generator=g, dtype=torch.int32)
+    steps[2:4] = steps[2:4].clamp(max=1)
+    steps[:, :, :20000] += 3
+    x = (top.view(torch.int32) - steps * torch.sign(top).int()).view(torch.float32).to(dev())
+    opts = options([1.0, 1.0, 1.0, 1.0, 0.9, 0.9, 1.4, 1.4], [0] * s, seed=62)
+    rows = [x[:, j].contiguous() for j in range(2)]
+    first = ops.sample(rows[0], *(opts[n] for n in NAMES))
+    second = ops.sample(rows[1], *(opts["step"] + 1 if n == "step" else opts[n] for n in NAMES))
+    got = ops.verify_drafts(x.reshape(2 * s, vocab), torch.stack((first, first), 1).flatten(), ints(range(0, 2 * s + 1, 2)), max_drafts=1, **opts)
+    assert got.tokens[:, 0].tolist() == first.tolist() and got.tokens[:, 1].tolist() == second.tolist() and got.counts.tolist() == [2] * s
