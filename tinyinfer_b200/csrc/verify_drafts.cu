@@ -914,8 +914,8 @@ TI_API int ti_verify_drafts(int* tokens, int* counts, float* accept, const float
     if (draft_logits) {
         constexpr int shared = VD_STAGES * 2 * VD_THREADS * 16;
         TI_REQUIRE((ti_allow_shared<verify_kernel<true, false>>(shared) == cudaSuccess), "verify_drafts: %d bytes of shared memory are not to be had", shared);
-        // Sixteen blocks a request while all of them run at once, otherwise eight: 32 requests x 4 drafts, of which 8 are open, 45 us for 49;
-        // 64 open requests x 7 drafts 146 us for 135.
+        // Sixteen blocks a request while all of them run at once, otherwise eight: 32 requests x 4 drafts, of which 8 are open, 40 us for 43;
+        // 64 open requests x 7 drafts 137 us for 126 (captured).
         const bool wide = requests * VD_MOST_CTAS <= 148 * 4 && ti_allow_wide_clusters<verify_kernel<true, false>>() == cudaSuccess;
         const int ctas = wide ? VD_MOST_CTAS : VD_CTAS;
         ti_launch_clusters(verify_kernel<true, false>, dim3(ctas, requests), ctas, VD_THREADS, shared, stream, a);
