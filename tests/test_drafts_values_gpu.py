@@ -71,7 +71,7 @@ def leftover_is_decided(row, dl, rel, temperature, topk, seed, stream, step):
     with np.errstate(divide="ignore"):
         least, most = np.log(np.maximum(left - off, 0.0)) + race, np.log(left + off) + race
     winner = int(np.argmax(np.log(left + 1e-300) + race))
-    return least[winner] > np.delete(most, winner).max()
+    return least[winner] > np.delete(most, winner).max(initial=-math.inf)
 
 
 def check(ops, x, fed, opts, q=None, allowed=None):
@@ -274,3 +274,32 @@ def test_where_the_noise_fades(ops, size):
     second = ops.sample(rows[1], *(opts["step"] + 1 if n == "step" else opts[n] for n in NAMES))
     got = ops.verify_drafts(x.reshape(2 * s, vocab), torch.stack((first, first), 1).flatten(), ints(range(0, 2 * s + 1, 2)), max_drafts=1, **opts)
     assert got.tokens[:, 0].tolist() == first.tolist() and got.tokens[:, 1].tolist() == second.tolist() and got.counts.tolist() == [2] * s
+
+
+@pytest.mark.parametrize("off", [0.0, 9e5, 3e6, -1.2e7])
+@pytest.mark.parametrize("topk", [0, 8])
+@pytest.mark.parametrize("which", [11, 17, 29])
+def test_tokens_are_distributed_as_the_target_says_far_from_0(ops, off, topk, which):
+    """40,000 requests with a draft each, drawn from q: the first tokens' frequencies are p's, whatever the roundings at the size of the
+    logits, which is the draft model's, too. With a threshold p and q are the softmax of the float32 quotients, without one of x / T. A
+    frequency is off by more than five standard deviations once in two million."""
+    v, n, t = 12, 40000, np.float32(0.9)
+    g = torch.Generator().manual_seed(which)
+    target, other = torch.randn(v, generator=g) * 1.5 + off, torch.randn(v, generator=g) * 1.5 + off
+
+    def softmax(x):
+        s = (x.numpy() / t).astype(np.float64) if topk else x.double().numpy() / float(t)
+        s[x.numpy() / t < np.sort(x.numpy() / t)[-(topk or v)]] = -math.inf
+        w = np.exp(s - s.max())
+        return w / w.sum()
+
+    p, q = softmax(target), softmax(other)
+    opts = options([float(t)] * n, [topk] * n, seed=6)
+    opts["seed"] = torch.full((n,), 1234, dtype=torch.int64, device=dev())
+    opts["stream_id"] = torch.arange(n, dtype=torch.int32, device=dev())
+    draft = torch.multinomial(torch.tensor(q), n, True, generator=g).int().to(dev())
+    fed = torch.stack((torch.zeros_like(draft), draft), 1).flatten().contiguous()
+    got = ops.verify_drafts(target.to(dev()).expand(2 * n, v).contiguous(), fed, torch.arange(0, 2 * n + 1, 2, dtype=torch.int32, device=dev()),
+                            max_drafts=1, draft_logits=other.to(dev()).expand(n, 1, v), **opts)
+    freq = np.bincount(got.tokens[:, 0].cpu().numpy(), minlength=v) / n
+    assert np.all(np.abs(freq - p) <= 5.0 * np.sqrt(p * (1 - p) / n) + 1e-9), (freq, p)

@@ -742,9 +742,10 @@ __global__ void __launch_bounds__(VD_THREADS, JUDGED ? 4 : 1) verify_kernel(VdAr
             const RowStats ds = failed ? row_sh[D + 1 + held] : RowStats{0.f, 0.f, 0u, -1, 0.f, -1, {0, 0}};
             const float* x = a.logits + (size_t)(rows.x + held) * a.vocab;
             const float* y = failed ? a.draft_logits + r * a.draft_request + held * a.draft_place : x;
-            Weights pw(temp, st.m);
-            const Weights qw(temp, ds.m);
-            pw.odd |= !failed && !pw.near();                 // a draw from p alone goes by the quotients
+            // By the quotients: rows with a threshold, whose sums were taken of them, and a draw from p alone far from 0, as sample's.
+            Weights pw(temp, st.m), qw(temp, ds.m);
+            pw.odd |= thresholded || (!failed && !pw.near());
+            qw.odd |= thresholded;
             const float pz = st.z > 0.f ? 1.f / st.z : 0.f, qz = ds.z > 0.f ? 1.f / ds.z : 0.f;
             auto p_of = [&](float v) { return v > -INFINITY && (!st.threshold || score_key(v / temp) >= st.threshold) ? pw(v) * pz : 0.f; };
             auto q_of = [&](float v) { return v > -INFINITY && (!ds.threshold || score_key(v / temp) >= ds.threshold) ? qw(v) * qz : 0.f; };

@@ -2459,6 +2459,7 @@ def verify_drafts(logits: torch.Tensor, token_ids: torch.Tensor, cu_rows: torch.
 
     The result's tensors share one allocation, with up to 1 MB that the call worked in: who keeps one of them for long keeps a copy of it.
 
+    Shares are float32: below 2^-126 they are 0, and a draft to which both models give less than that, which none could draw, does not hold.
     A draft outside the vocabulary never holds. NaN logits are passed over, as ``sample`` does; a sampled row with nothing but NaN and
     -inf, or whose quotients by the temperature are all -inf, lets no draft hold and gives token 0. One thing differs from ``sample``: at the
     top-k threshold -0 and +0 are one value here, so that both are kept, where ``sample`` takes -0 for the lower."""
